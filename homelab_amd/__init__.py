@@ -17,6 +17,8 @@ OK = 0
 ERR_ARG, ERR_WORKSPACE, ERR_LAUNCH, ERR_KERNEL = -1, -2, -3, -4
 F32, BF16 = 0, 1
 SCALE_ROW, SCALE_1X128, SCALE_128X128 = 0, 1, 2
+ROPE_HALF, ROPE_INTERLEAVED = 0, 1  # pairs (i, i + rot / 2) or (2i, 2i + 1)
+ROPE_PLAIN, ROPE_LINEAR, ROPE_YARN = 0, 1, 2  # how the frequencies are scaled
 EXPERT_EXACT, EXPERT_BF16 = 0, 1  # the prefill down projection's activation precision
 
 _lib = None
@@ -31,6 +33,14 @@ class Fp8Record(ctypes.Structure):
 
     _fields_ = [(n, ctypes.c_int64) for n in (
         "hidden", "inter", "gate_weight", "gate_scale", "up_weight", "up_scale", "down_weight", "down_scale")]
+
+
+class Rope(ctypes.Structure):
+    """OomRope: what a model's configuration says of its rotary positions."""
+
+    _fields_ = [("rot_dim", ctypes.c_int64), ("scaling", ctypes.c_int64), ("base", ctypes.c_double),
+                ("factor", ctypes.c_double), ("trained_len", ctypes.c_int64), ("beta_fast", ctypes.c_double),
+                ("beta_slow", ctypes.c_double)]
 
 
 # entry point -> (restype, argtypes); every symbol include/oom_hip.h declares
@@ -81,6 +91,16 @@ SIGNATURES = {
     "oom_mask_compact": (I32, [P, P, I32, P]),
     "oom_attn_decode_turbo_workspace_size": (SZ, [I32, I32, I32, I32]),
     "oom_attn_decode_turbo": (I32, [P, P, P, I32, I32, P, P, I32, I32, I32, I32, F, P, P, SZ, P]),
+    "oom_rope_table": (I32, [P, P, SZ, P]),
+    "oom_rope": (I32, [P, I32, I64, P, P, I32, I32, F, I32, P, I32, I64, I32, I32, I32, P]),
+    "oom_rope_append_paged": (I32, [P, I64, P, I64, P, I64, I32, P, P, P, I32, I32, F, P, I32, I64, P, P, I32, I32,
+                                    I32, I32, I32, I32, P]),
+    "oom_attn_plan_size": (SZ, [I32, I32, I32, I32, I32]),
+    "oom_attn_plan": (I32, [P, P, P, I32, I32, I32, I32, I32, I32, I32, I32, P, P, P, P]),
+    "oom_attn_prompt": (I32, [P, I32, I64, P, I64, P, I64, P, I32, I32, I32, I32, I32, F, P, I32, I64, P]),
+    "oom_attn_chunk_paged_workspace_size": (SZ, [I32, I32, I32, I32, I32]),
+    "oom_attn_chunk_paged": (I32, [P, I32, I64, P, P, P, I32, I32, I32, P, I32, I32, I32, I32, I32, I32, F, P, I32, I64,
+                                   P, SZ, P]),
     "oom_copy_queue_create": (I32, [P]),
     "oom_copy_queue_destroy": (I32, [P]),
     "oom_host_alloc": (I32, [P, SZ]),
@@ -414,6 +434,179 @@ def attn_decode_turbo(q, k, v, k_bits: int, v_bits: int, levels, mask, kv_heads:
     check(lib().oom_attn_decode_turbo(_ptr(q), _ptr(k), _ptr(v), k_bits, v_bits, _ptr(levels), _ptr(mask), heads,
                                       kv_heads, d, kv_len, scale, _ptr(out), _ptr(ws), ws.numel() * ws.element_size(),
                                       _stream(stream)))
+
+
+# ---- the prompt path: rotary positions, paged cache writes, prompt and chunk attention ----
+
+def _need(ok: bool, msg: str) -> None:
+    if not ok:
+        raise OomError(msg)
+
+
+def _on_device(name: str, stream, **tensors):
+    """The stream of a call: `stream`, or the tensors' device's current one. Every tensor is on
+    that device."""
+    import torch
+
+    dev = None
+    for what, t in tensors.items():
+        if t is None:
+            continue
+        _need(t.is_cuda, f"{name}: {what} is not on the GPU")
+        dev = dev or t.device
+        _need(t.device == dev, f"{name}: {what} is on {t.device}, not on {dev}")
+    s = stream if stream is not None else torch.cuda.current_stream(dev)
+    _need(s.device == dev, f"{name}: the stream is of {s.device}, the tensors are on {dev}")
+    return torch.cuda.device(dev), ctypes.c_void_p(s.cuda_stream)
+
+
+def _rows(name: str, what: str, t, d: int | None = None) -> int:
+    """The token stride of rows [T, heads, d] whose heads lie side by side."""
+    _need(t.dim() == 3, f"{name}: {what} must be [tokens, heads, d]")
+    T, heads, dd = t.shape
+    _need(d is None or dd == d, f"{name}: {what} has head_dim {dd}, not {d}")
+    _need((dd == 1 or t.stride(2) == 1) and (heads == 1 or t.stride(1) == dd),
+          f"{name}: the heads of a token of {what} must be contiguous")
+    return t.stride(0) if T > 1 else heads * dd
+
+
+def _flat(name: str, what: str, t, dtype: str, n: int | None = None) -> None:
+    """A contiguous tensor of a type; n: its least number of elements."""
+    _need(str(t.dtype) == "torch." + dtype and t.is_contiguous(), f"{name}: {what} must be a contiguous {dtype} tensor")
+    _need(n is None or t.numel() >= n, f"{name}: {what} holds {t.numel()} elements, {n} are needed")
+
+
+def _pages(name: str, k_pages, v_pages, kv_heads: int, d: int):
+    """(n_pages, page_size) of a cache [n_pages, kv_heads, page_size, d]."""
+    _flat(name, "k_pages", k_pages, "bfloat16")
+    _flat(name, "v_pages", v_pages, "bfloat16")
+    _need(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.shape[1] == kv_heads and
+          k_pages.shape[3] == d, f"{name}: k_pages and v_pages must be [n_pages, {kv_heads}, page_size, {d}]")
+    return k_pages.shape[0], k_pages.shape[2]
+
+
+def rope_table(rot_dim: int, base: float = 10000.0, scaling: int = ROPE_PLAIN, factor: float = 1.0,
+               trained_len: int = 0, beta_fast: float = 32.0, beta_slow: float = 1.0):
+    """(turns, magnitude): the frequency table (numpy u64 [rot_dim / 2], for the device as the
+    int64 view of the same bits) and the factor on cos and sin."""
+    import numpy as np
+
+    cfg = Rope(rot_dim, scaling, base, factor, trained_len, beta_fast, beta_slow)
+    turns = np.empty(max(1, rot_dim // 2), dtype=np.uint64)
+    mag = ctypes.c_float()
+    check(lib().oom_rope_table(ctypes.byref(cfg), turns.ctypes.data_as(ctypes.c_void_p), turns.size,
+                               ctypes.byref(mag)))
+    return turns, mag.value
+
+
+def rope(x, positions, turns, out, layout: int = ROPE_HALF, magnitude: float = 1.0, inverse: bool = False,
+         stream=None) -> None:
+    """Rotary positions of x [T, heads, d] into out (which may be x); positions i32 [T]; turns int64
+    [rot_dim / 2], the device copy of rope_table's."""
+    T, heads, d = x.shape
+    xs, os = _rows("rope", "x", x), _rows("rope", "out", out, d)
+    _need(out.shape == x.shape, "rope: out must have x's shape")
+    _flat("rope", "positions", positions, "int32", T)
+    _flat("rope", "turns", turns, "int64", 1)
+    dev, st = _on_device("rope", stream, x=x, positions=positions, turns=turns, out=out)
+    with dev:
+        check(lib().oom_rope(_ptr(x), _dtype_code(x), xs, _ptr(positions), _ptr(turns), 2 * turns.numel(), layout,
+                             magnitude, int(inverse), _ptr(out), _dtype_code(out), os, T, heads, d, st))
+
+
+def rope_append_paged(q, k, v, positions, slots, turns, q_out, k_pages, v_pages, layout: int = ROPE_HALF,
+                      magnitude: float = 1.0, stream=None) -> None:
+    """q [T, heads, d] rotated into q_out (which may be q), k [T, kv_heads, d] rotated and v as it is
+    into the cache slots slots i64 [T]."""
+    name = "rope_append_paged"
+    T, heads, d = q.shape
+    qs, ks, vs, os = (_rows(name, w, t, d) for w, t in (("q", q), ("k", k), ("v", v), ("q_out", q_out)))
+    _need(q_out.shape == q.shape and k.shape == v.shape and k.shape[0] == T, f"{name}: q_out must have q's shape, v k's")
+    _need(q.dtype == k.dtype == v.dtype, f"{name}: q, k and v must have one type")
+    _flat(name, "positions", positions, "int32", T)
+    _flat(name, "slots", slots, "int64", T)
+    _flat(name, "turns", turns, "int64", 1)
+    n_pages, ps = _pages(name, k_pages, v_pages, k.shape[1], d)
+    dev, st = _on_device(name, stream, q=q, k=k, v=v, positions=positions, slots=slots, turns=turns, q_out=q_out,
+                         k_pages=k_pages, v_pages=v_pages)
+    with dev:
+        check(lib().oom_rope_append_paged(_ptr(q), qs, _ptr(k), ks, _ptr(v), vs, _dtype_code(q), _ptr(positions),
+                                          _ptr(slots), _ptr(turns), 2 * turns.numel(), layout, magnitude, _ptr(q_out),
+                                          _dtype_code(q_out), os, _ptr(k_pages), _ptr(v_pages), n_pages, ps, T, heads,
+                                          k.shape[1], d, st))
+
+
+def attn_plan_size(T: int, B: int, heads: int, kv_heads: int, d: int) -> int:
+    return int(lib().oom_attn_plan_size(T, B, heads, kv_heads, d))
+
+
+def attn_plan(cu_q, kv_lens, page_table, T: int, heads: int, kv_heads: int, d: int, plan, n_pages: int = 0,
+              page_size: int = 0, positions=None, slots=None, stream=None) -> None:
+    """The plan of a step's batch: cu_q i32 [B + 1]; kv_lens i32 [B] and page_table i32 [B, max_pages]
+    of a cache of n_pages pages, or None for prompts; plan i32 [attn_plan_size()]."""
+    B = cu_q.numel() - 1
+    _need(B >= 0, "attn_plan: cu_q must hold B + 1 elements")
+    _flat("attn_plan", "cu_q", cu_q, "int32")
+    _flat("attn_plan", "plan", plan, "int32", attn_plan_size(T, B, heads, kv_heads, d))
+    max_pages = 0
+    if page_table is not None:
+        _flat("attn_plan", "page_table", page_table, "int32")
+        _need(page_table.dim() == 2 and page_table.shape[0] == B, "attn_plan: page_table must be [B, max_pages]")
+        max_pages = page_table.shape[1]
+    if kv_lens is not None:
+        _flat("attn_plan", "kv_lens", kv_lens, "int32", B)
+    if positions is not None:
+        _flat("attn_plan", "positions", positions, "int32", T)
+    if slots is not None:
+        _flat("attn_plan", "slots", slots, "int64", T)
+    dev, st = _on_device("attn_plan", stream, cu_q=cu_q, kv_lens=kv_lens, page_table=page_table, plan=plan,
+                         positions=positions, slots=slots)
+    with dev:
+        check(lib().oom_attn_plan(_ptr(cu_q), _ptr(kv_lens), _ptr(page_table), max_pages, n_pages, page_size, T, B,
+                                  heads, kv_heads, d, _ptr(positions), _ptr(slots), _ptr(plan), st))
+
+
+def attn_prompt(q, k, v, plan, B: int, scale: float, out, stream=None) -> None:
+    """Causal attention of B packed prompts: q [T, heads, d]; k and v bf16 [T, kv_heads, d]; plan
+    attn_plan's without kv_lens."""
+    import torch
+
+    name = "attn_prompt"
+    T, heads, d = q.shape
+    qs, ks, vs, os = (_rows(name, w, t, d) for w, t in (("q", q), ("k", k), ("v", v), ("out", out)))
+    _need(out.shape == q.shape and k.shape == v.shape and k.shape[0] == T, f"{name}: out must have q's shape, v k's")
+    _need(k.dtype == v.dtype == torch.bfloat16, f"{name}: k and v must be bfloat16")
+    _flat(name, "plan", plan, "int32", attn_plan_size(T, B, heads, k.shape[1], d))
+    dev, st = _on_device(name, stream, q=q, k=k, v=v, plan=plan, out=out)
+    with dev:
+        check(lib().oom_attn_prompt(_ptr(q), _dtype_code(q), qs, _ptr(k), ks, _ptr(v), vs, _ptr(plan), T, B, heads,
+                                    k.shape[1], d, scale, _ptr(out), _dtype_code(out), os, st))
+
+
+def attn_chunk_paged_workspace_size(T: int, B: int, heads: int, kv_heads: int, d: int) -> int:
+    return int(lib().oom_attn_chunk_paged_workspace_size(T, B, heads, kv_heads, d))
+
+
+def attn_chunk_paged(q, k_pages, v_pages, page_table, plan, max_q: int, scale: float, out, ws, stream=None) -> None:
+    """New tokens q [T, heads, d] over the paged cache; page_table i32 [B, max_pages]; plan attn_plan's
+    with the same table; max_q: the most new tokens of any sequence."""
+    name = "attn_chunk_paged"
+    T, heads, d = q.shape
+    qs, os = _rows(name, "q", q), _rows(name, "out", out, d)
+    _need(out.shape == q.shape, f"{name}: out must have q's shape")
+    _need(k_pages.dim() == 4, f"{name}: k_pages must be [n_pages, kv_heads, page_size, d]")
+    kv_heads = k_pages.shape[1]
+    n_pages, ps = _pages(name, k_pages, v_pages, kv_heads, d)
+    _flat(name, "page_table", page_table, "int32")
+    _need(page_table.dim() == 2, f"{name}: page_table must be [B, max_pages]")
+    B, max_pages = page_table.shape
+    _flat(name, "plan", plan, "int32", attn_plan_size(T, B, heads, kv_heads, d))
+    dev, st = _on_device(name, stream, q=q, k_pages=k_pages, v_pages=v_pages, page_table=page_table, plan=plan, out=out,
+                         ws=ws)
+    with dev:
+        check(lib().oom_attn_chunk_paged(_ptr(q), _dtype_code(q), qs, _ptr(k_pages), _ptr(v_pages), _ptr(page_table),
+                                         max_pages, n_pages, ps, _ptr(plan), T, B, max_q, heads, kv_heads, d, scale,
+                                         _ptr(out), _dtype_code(out), os, _ptr(ws), ws.numel() * ws.element_size(), st))
 
 
 def quantize_rows_fp8(x, q, scale, stream=None) -> None:

@@ -1,0 +1,497 @@
+// Attention of tiles of query rows over 64-key tiles in LDS: the device core of
+// oom_attn_prompt (packed prompts, K and V rows as the projections wrote them) and
+// oom_attn_chunk_paged (new tokens over paged caches).
+//
+// A row is one (token, query head) pair: the G query heads that share a KV head are packed
+// beside each other, row t G + g, so every row of a tile reads the same K and V and the
+// rows of a tile span few tokens, whose causal bounds nearly agree.
+//
+//  * Scores S^T = K Q^T on v_mfma_f32_32x32x16_bf16 (keys on M): lane l ends with 16 keys of
+//    row l % 32 a 32-key step, so the softmax of a row stays inside two lanes; its maximum
+//    costs one half-wave swap a tile and its sum none before the end.
+//  * O^T = V^T P^T on the same instruction (dims on M). The keys of a product may be summed
+//    in any order that both operands share: P stays in the registers where the scores left
+//    it, and V takes that order through transposing LDS reads (ds_read_b64_tr_b16, four keys
+//    of one dim a lane).
+//  * Running maximum m and sum l in fp32, base-2 exponentials: p = 2^(s c - m c), c = scale
+//    log2 e, one fused multiply-add; for c > 1, where a finite score times c may be infinite, 2^((s -
+//    m) c). O is rescaled only when some row's maximum grew by more than a factor of 2^8: until
+//    then the older maximum keeps every p below 2^8, which fp32 sums hold as well.
+#pragma once
+
+#include "common.hpp"
+
+namespace oom {
+
+typedef __bf16 tbf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 tbf16x2 __attribute__((ext_vector_type(2)));
+typedef float tf32x2 __attribute__((ext_vector_type(2)));
+typedef float tf32x16 __attribute__((ext_vector_type(16)));
+typedef short ts16x4 __attribute__((ext_vector_type(4)));
+typedef __attribute__((address_space(3))) ts16x4* tr_ptr_t;
+typedef __attribute__((address_space(3))) void* t_lds_t;
+typedef const __attribute__((address_space(1))) void* t_glb_t;
+
+constexpr float T_GROW = 8.0f;  // growth of a row's maximum (log2) that rescales O
+
+// What one block works on: an entry of the plan (attn_plan.hip).
+struct AttnItem {
+    int q0;    // first token row of the sequence
+    int row0;  // first packed row of the tile within the sequence
+    int rows;  // its rows
+    int off;   // position of the sequence's first new token
+    int k0, k1;  // its keys [k0, k1), k0 a multiple of 64
+    int part;  // first row of its partial, -1: the only split, writes out
+    int seq;
+};
+static_assert(sizeof(AttnItem) == 4 * ATTN_ITEM_WORDS, "plan item");
+
+struct TileArgs {
+    const void* q;
+    int64_t q_stride;  // elements between tokens
+    int q_dtype, out_dtype;
+    void* out;
+    int64_t out_stride;
+    const uint16_t* k;  // prompt: rows [T, Hkv, d]; paged: the pages
+    const uint16_t* v;
+    int64_t k_stride, v_stride;  // prompt: elements between tokens
+    const int32_t* table;        // paged: [B, max_pages]
+    int max_pages, n_pages, page_size;
+    const int32_t* plan;
+    int G, Hkv;
+    float scale;
+    float* part_ml;   // [Hkv][part rows][2]: maximum score and sum
+    float* part_acc;  // [Hkv][part rows][d]
+    int64_t part_rows;
+};
+
+// Rows that a bad page index, or a key past the item's end, reads: zeros.
+static __device__ __align__(16) uint16_t t_zero_row[256];
+
+__device__ __forceinline__ uint32_t t_pack(float a, float b) {
+    const tf32x2 f = {a, b};
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector(f, tbf16x2));  // RNE
+}
+
+__device__ __forceinline__ void t_barrier() {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_barrier();
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
+// A K or V tile in LDS: 64 rows (keys) of d bf16, in 16-byte chunks, C = d / 8 a row, each row's
+// chunks permuted by an exclusive or with a value of the row, so that the lanes of a read,
+// which take the same chunks of consecutive rows, meet different banks. A direct-to-LDS load
+// writes lane l's 16 bytes at its base + 16 l, so the permutation is in the global addresses.
+//   K: chunk ^ (row % 16 (8 for d = 64)): 16 consecutive rows' same chunk in 16 places
+//   V: the transposing read takes 4 rows x 2 chunks a 16-lane group
+template <int D>
+struct TileLay {
+    static constexpr int C = D / 8, ROWB = D * 2, BYTES = 64 * ROWB;
+    static constexpr int RPI = 64 / C;  // rows an instruction loads
+    static __device__ __forceinline__ int kx(int row) { return row & (C < 16 ? C - 1 : 15); }
+    static __device__ __forceinline__ int vx(int row) { return D == 64 ? ((row >> 1) & 1) * 2 : (row & 3) * 4; }
+};
+
+// Loads of one 64-key tile: wave w of 4 takes rows 16 w .. 16 w + 15 of K and of V, which lie in
+// one page.
+template <int D, bool PAGED>
+struct TileSrc {
+    typedef TileLay<D> L;
+    static constexpr int NI = 16 / L::RPI;  // instructions a wave
+    const uint16_t *k, *v;
+    int64_t ks, vs;  // elements between rows
+    const int32_t* table;
+    int n_pages, p16, head, k1;
+    int64_t page_elems;
+    int ko[NI], vo;  // byte offsets of this lane from the wave's first row
+
+    __device__ __forceinline__ void init(const TileArgs& a, const AttnItem& it, int h, int lane) {
+        k1 = it.k1;
+        if constexpr (PAGED) {
+            ks = vs = D;
+            k = a.k;
+            v = a.v;
+            table = a.table + (size_t)it.seq * a.max_pages;
+            n_pages = a.n_pages;
+            p16 = a.page_size / 16;
+            head = h;
+            page_elems = (int64_t)a.page_size * a.Hkv * D;
+        } else {
+            ks = a.k_stride;
+            vs = a.v_stride;
+            k = a.k + (int64_t)it.q0 * ks + h * D;
+            v = a.v + (int64_t)it.q0 * vs + h * D;
+        }
+        const int r = lane / L::C, c = lane % L::C;
+#pragma unroll
+        for (int n = 0; n < NI; n++) ko[n] = (int)((n * L::RPI + r) * ks * 2) + 16 * (c ^ L::kx(n * L::RPI + r));
+        vo = (int)(r * vs * 2) + 16 * (c ^ L::vx(r));
+        static_assert(L::RPI % 4 == 0 || L::RPI == 2, "V's permutation per instruction");
+    }
+
+    // The wave's 16 rows from key `key` (a multiple of 16) on into its places kt and vt (the
+    // tiles + 16 w rows).
+    __device__ __forceinline__ void load(int key, int lane, uint8_t* kt, uint8_t* vt) const {
+        const uint16_t *kb = nullptr, *vb = nullptr;
+        bool ok = key < k1;
+        if constexpr (PAGED) {
+            if (ok) {
+                const uint32_t sub = (uint32_t)key / 16, pi = sub / (uint32_t)p16, si = sub - pi * p16;
+                const int page = table[pi];
+                ok = page >= 0 && page < n_pages;
+                const int64_t at = (ok ? page : 0) * page_elems + ((int64_t)head * p16 + si) * 16 * D;
+                kb = k + at;
+                vb = v + at;
+            }
+        } else {
+            kb = k + key * ks;
+            vb = v + key * vs;
+        }
+        if (ok && key + 16 <= k1) {  // uniform
+#pragma unroll
+            for (int n = 0; n < NI; n++)
+                __builtin_amdgcn_global_load_lds((t_glb_t)((const uint8_t*)kb + ko[n]),
+                                                 (t_lds_t)(kt + n * 1024), 16, 0, 0);
+#pragma unroll
+            for (int n = 0; n < NI; n++)
+                __builtin_amdgcn_global_load_lds((t_glb_t)((const uint8_t*)vb + v_off(n, lane)),
+                                                 (t_lds_t)(vt + n * 1024), 16, 0, 0);
+            return;
+        }
+        const int r = lane / L::C, c = lane % L::C;
+        const uint8_t* z = (const uint8_t*)t_zero_row + 16 * c;
+#pragma unroll
+        for (int n = 0; n < NI; n++) {
+            const bool in = ok && key + n * L::RPI + r < k1;
+            __builtin_amdgcn_global_load_lds((t_glb_t)(in ? (const uint8_t*)kb + ko[n] : z), (t_lds_t)(kt + n * 1024),
+                                             16, 0, 0);
+            __builtin_amdgcn_global_load_lds((t_glb_t)(in ? (const uint8_t*)vb + v_off(n, lane) : z),
+                                             (t_lds_t)(vt + n * 1024), 16, 0, 0);
+        }
+    }
+
+    __device__ __forceinline__ int64_t v_off(int n, int lane) const {
+        // rows of instruction n are n RPI + lane / C: with RPI a multiple of 4 the permutation does
+        // not depend on n; with two rows an instruction it alternates
+        if constexpr (L::RPI % 4 == 0) return vo + (int64_t)n * L::RPI * vs * 2;
+        const int r = lane / L::C, c = lane % L::C;
+        return (n * L::RPI + r) * vs * 2 + 16 * (c ^ L::vx(n * L::RPI + r));
+    }
+};
+
+// bf16 pairs whose exponent is all ones (infinity or NaN) in either half: nonzero.
+__device__ __forceinline__ uint32_t t_nonfinite(uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+// The pair with such halves cleared.
+__device__ __forceinline__ uint32_t t_finite(uint32_t w) {
+    const uint32_t b = t_nonfinite(w);
+    uint32_t m = (b >> 15) * 0xffffu;  // 0x00010001 flags to half masks
+    return w & ~m;
+}
+
+// TERMS 1: bf16 queries and outputs: the products take Q as it is and P rounded to bf16 (its
+// relative error, at most 2^-8 a key and averaged over the keys, is of the size of the
+// output's own rounding). TERMS 3: fp32 on either side: Q and P enter as three exact bf16
+// terms each (hi + mid + lo), so products are exact and only fp32 sums round.
+template <int D, int TERMS>
+struct RowState {
+    tbf16x8 q[TERMS][D / 16];
+    tf32x16 o[D / 32];
+    float m, l;
+    int pos;    // the last key this lane's row sees
+    bool live;  // the lane has a row
+};
+
+template <int D, int TERMS>
+__device__ __forceinline__ void rows_init(RowState<D, TERMS>& s, const TileArgs& a, const AttnItem& it, int h, int wrow,
+                                          int lane) {
+    const int r = wrow + (lane & 31), half = lane >> 5;
+    s.live = r < it.rows;
+    const uint32_t row = (uint32_t)(it.row0 + (s.live ? r : 0)), tok = row / (uint32_t)a.G, g = row - tok * a.G;
+    s.pos = it.off + (int)tok;
+    s.m = -INFINITY;
+    s.l = 0.0f;
+#pragma unroll
+    for (int d = 0; d < D / 32; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) s.o[d][i] = 0.0f;
+    const int64_t at = (int64_t)(it.q0 + (int)tok) * a.q_stride + (int64_t)(h * a.G + (int)g) * D + 8 * half;
+    if (a.q_dtype == OOM_BF16) {
+        const uint16_t* p = reinterpret_cast<const uint16_t*>(a.q) + at;
+#pragma unroll
+        for (int c = 0; c < D / 16; c++) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p + 16 * c);
+            s.q[0][c] = __builtin_bit_cast(tbf16x8, v);
+            if constexpr (TERMS == 3)
+                s.q[1][c] = s.q[2][c] = __builtin_bit_cast(tbf16x8, make_uint4(0, 0, 0, 0));
+        }
+    } else if constexpr (TERMS == 3) {
+        const float* p = reinterpret_cast<const float*>(a.q) + at;
+#pragma unroll
+        for (int c = 0; c < D / 16; c++) {
+            const float4 v0 = *reinterpret_cast<const float4*>(p + 16 * c);
+            const float4 v1 = *reinterpret_cast<const float4*>(p + 16 * c + 4);
+            float f[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+#pragma unroll
+            for (int t = 0; t < 3; t++) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    w[e] = t_pack(f[2 * e], f[2 * e + 1]);
+                    f[2 * e] -= __uint_as_float(w[e] << 16);  // exact: the remainder of a round to nearest
+                    f[2 * e + 1] -= __uint_as_float(w[e] & 0xffff0000u);
+                }
+                s.q[t][c] = __builtin_bit_cast(tbf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+            }
+        }
+    }
+}
+
+__device__ __forceinline__ tbf16x8 t_finite8(tbf16x8 v) {
+    const uint4 w = __builtin_bit_cast(uint4, v);
+    return __builtin_bit_cast(tbf16x8, make_uint4(t_finite(w.x), t_finite(w.y), t_finite(w.z), t_finite(w.w)));
+}
+
+// One 64-key tile from LDS. MASKED: some key of the tile is hidden from some row (a later
+// position, or past the item's keys), and V may hold infinities or NaN there (bad_v): those are
+// taken out of the product and added to the rows that see them. With three terms, an infinity of
+// K (bad_k) or V meets the first alone: the others may be zero or of the other sign.
+template <int D, int TERMS, bool MASKED>
+__device__ __forceinline__ void tile_step(RowState<D, TERMS>& s, const uint8_t* kt, const uint8_t* vt, int key0, int k1,
+                                          float c, bool bad_k, bool bad_v, int lane) {
+    typedef TileLay<D> L;
+    const int half = lane >> 5;
+    // ---- scores: 32 keys at a time; lane: key 32 n + 8 (i / 4) + 4 half + i % 4 of row l % 32 ----
+    tf32x16 sc[2];
+    const uint8_t* krow = kt + (lane & 31) * L::ROWB;
+    const int kx = L::kx(lane & 31);
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+#pragma unroll
+        for (int i = 0; i < 16; i++) sc[n][i] = 0.0f;
+#pragma unroll
+        for (int st = 0; st < D / 16; st++) {
+            const uint4 kv = *reinterpret_cast<const uint4*>(krow + 32 * n * L::ROWB + 16 * ((2 * st + half) ^ kx));
+            const tbf16x8 ka = __builtin_bit_cast(tbf16x8, kv);
+            if constexpr (TERMS > 1) {
+                const tbf16x8 kf = bad_k ? t_finite8(ka) : ka;
+#pragma unroll
+                for (int t = TERMS - 1; t > 0; t--)
+                    sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, s.q[t][st], sc[n], 0, 0, 0);
+            }
+            sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, s.q[0][st], sc[n], 0, 0, 0);
+        }
+    }
+    if constexpr (MASKED) {
+        const int last = min(s.pos, k1 - 1) - key0;
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int i = 0; i < 16; i++)
+                if (32 * n + 8 * (i / 4) + 4 * half + i % 4 > last) sc[n][i] = -INFINITY;
+    }
+    // ---- running maximum ----
+    float mx = sc[0][0];
+#pragma unroll
+    for (int n = 0; n < 2; n++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) mx = fmaxf(mx, sc[n][i]);
+    {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    if (__any((mx - s.m) * c > T_GROW || s.m == -INFINITY)) {
+        const float mn = fmaxf(s.m, mx);
+        const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((s.m - mn) * c);
+        s.m = mn;
+        s.l *= f;
+#pragma unroll
+        for (int d = 0; d < D / 32; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) s.o[d][i] *= f;
+    }
+    const float m0 = s.m == -INFINITY ? 0.0f : s.m, mb = m0 * c;
+    // ---- p, its sum, and the products, 16 keys at a time ----
+    const int grp = lane >> 4, r4 = (lane & 15) >> 2;
+    const uint8_t* vrow = vt + (4 * half + r4) * L::ROWB + 8 * (lane & 1);
+    const int vc = 2 * (grp & 1) + ((lane & 3) >> 1), vx = L::vx(4 * half + r4);
+#pragma unroll
+    for (int n = 0; n < 2; n++) {
+        float p[16], sum = 0.0f;
+        if (c <= 1.0f) {  // uniform
+#pragma unroll
+            for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[n][i], c, -mb));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f((sc[n][i] - m0) * c);
+        }
+#pragma unroll
+        for (int i = 0; i < 16; i++) sum += p[i];
+        s.l += sum;
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            tbf16x8 pb[TERMS];
+#pragma unroll
+            for (int t = 0; t < TERMS; t++) {
+                uint32_t w[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float &x = p[8 * u + 2 * e], &y = p[8 * u + 2 * e + 1];
+                    w[e] = t_pack(x, y);
+                    if (t + 1 < TERMS) {
+                        x -= __uint_as_float(w[e] << 16);
+                        y -= __uint_as_float(w[e] & 0xffff0000u);
+                    }
+                }
+                pb[t] = __builtin_bit_cast(tbf16x8, make_uint4(w[0], w[1], w[2], w[3]));
+            }
+#pragma unroll
+            for (int d = 0; d < D / 32; d++) {
+                const uint8_t* va = vrow + (32 * n + 16 * u) * L::ROWB + 16 * ((4 * d + vc) ^ vx);
+                const ts16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)va);
+                const ts16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(va + 8 * L::ROWB));
+                const uint2 w0 = __builtin_bit_cast(uint2, v0), w1 = __builtin_bit_cast(uint2, v1);
+                const tbf16x8 vv = __builtin_bit_cast(tbf16x8, make_uint4(w0.x, w0.y, w1.x, w1.y));
+                tbf16x8 vf = vv;
+                if constexpr (MASKED || TERMS > 1) vf = bad_v ? t_finite8(vv) : vv;
+#pragma unroll
+                for (int t = TERMS - 1; t >= 0; t--)
+                    s.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(MASKED || t > 0 ? vf : vv, pb[t], s.o[d], 0, 0, 0);
+            }
+        }
+    }
+    if constexpr (MASKED) {
+        if (bad_v) {  // uniform; rare: infinities and NaN of V reach the rows that see their key
+            const int last = min(s.pos, k1 - 1) - key0;
+            for (int key = 0; key < 64; key++) {
+                if (!__any(key <= last)) break;
+#pragma unroll
+                for (int d = 0; d < D / 32; d++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const int chunk = (4 * d + e) ^ L::vx(key);  // dims 32 d + 8 e + 4 half ..
+                        const uint2 w = *reinterpret_cast<const uint2*>(vt + key * L::ROWB + 16 * chunk + 8 * half);
+                        const uint32_t b0 = w.x & ~t_finite(w.x), b1 = w.y & ~t_finite(w.y);
+                        if (key <= last) {
+                            s.o[d][4 * e] += __uint_as_float(b0 << 16);
+                            s.o[d][4 * e + 1] += __uint_as_float(b0 & 0xffff0000u);
+                            s.o[d][4 * e + 2] += __uint_as_float(b1 << 16);
+                            s.o[d][4 * e + 3] += __uint_as_float(b1 & 0xffff0000u);
+                        }
+                    }
+            }
+        }
+    }
+}
+
+// out = O / l of the wave's rows, or their partial (O, m, l) for the merge. A row that sees no key
+// gives zeros.
+template <int D, int TERMS>
+__device__ __forceinline__ void rows_store(RowState<D, TERMS>& s, const TileArgs& a, const AttnItem& it, int h, int wrow,
+                                           int lane) {
+    const int r = wrow + (lane & 31), half = lane >> 5;
+    {
+        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(s.l), __float_as_uint(s.l), false, false);
+        s.l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
+    }
+    if (!s.live) return;
+    if (it.part >= 0) {
+        const int64_t pr = (int64_t)h * a.part_rows + it.part + r;
+        if (half == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * pr) = make_float2(s.m, s.l);
+#pragma unroll
+        for (int d = 0; d < D / 32; d++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                *reinterpret_cast<float4*>(a.part_acc + pr * D + 32 * d + 8 * e + 4 * half) =
+                    make_float4(s.o[d][4 * e], s.o[d][4 * e + 1], s.o[d][4 * e + 2], s.o[d][4 * e + 3]);
+        return;
+    }
+    const float inv = s.pos < 0 ? 0.0f : 1.0f / s.l;
+    const uint32_t row = (uint32_t)(it.row0 + r), tok = row / (uint32_t)a.G, g = row - tok * a.G;
+    const int64_t at = (int64_t)(it.q0 + (int)tok) * a.out_stride + (int64_t)(h * a.G + (int)g) * D + 4 * half;
+#pragma unroll
+    for (int d = 0; d < D / 32; d++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float x0 = s.o[d][4 * e] * inv, x1 = s.o[d][4 * e + 1] * inv, x2 = s.o[d][4 * e + 2] * inv,
+                        x3 = s.o[d][4 * e + 3] * inv;
+            const int64_t i = at + 32 * d + 8 * e;
+            if (a.out_dtype == OOM_BF16)
+                *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + i) = make_uint2(t_pack(x0, x1), t_pack(x2, x3));
+            else
+                *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + i) = make_float4(x0, x1, x2, x3);
+        }
+}
+
+// Blocks of 4 waves, 32 rows each; block i takes item i / Hkv for KV head i % Hkv (consecutive
+// blocks run on different XCDs, so with 8 KV heads each L2 holds one head's K and V).
+// K and V tiles go through LDS in two stages, one barrier a tile: past it, every wave has done
+// with the stage that the next tile's loads now fill, and those have a whole tile to arrive.
+template <int D, int TERMS, bool PAGED>
+__global__ void __launch_bounds__(256, (D <= 128 && TERMS == 1) ? 2 : 1) attn_tile_kernel(TileArgs a) {
+    typedef TileLay<D> L;
+    // each stage its own LDS object, so the compiler's waits for direct-to-LDS loads cover only the
+    // loads into the buffer a read touches
+    __shared__ __align__(16) uint8_t kt0[L::BYTES], vt0[L::BYTES], kt1[L::BYTES], vt1[L::BYTES];
+    __shared__ uint32_t bad_lds[4];  // per stage: K, V hold infinities or NaN
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = (int)(blockIdx.x % (uint32_t)a.Hkv), item = (int)(blockIdx.x / (uint32_t)a.Hkv);
+    if (item >= a.plan[ATTN_PLAN_ITEMS]) return;
+    const AttnItem it = reinterpret_cast<const AttnItem*>(a.plan + ATTN_PLAN_HEAD)[item];
+    const int wrow = 32 * wave;
+    const bool has = wrow < it.rows;  // uniform
+    const float c = a.scale * 1.44269504088896340736f;
+    TileSrc<D, PAGED> src;
+    src.init(a, it, h, lane);
+    if (threadIdx.x < 4) bad_lds[threadIdx.x] = 0;
+    RowState<D, TERMS> s;
+    rows_init(s, a, it, h, wrow, lane);
+    // positions of the wave's first and last row
+    const int pos_lo = it.off + (int)((uint32_t)(it.row0 + min(wrow, it.rows - 1)) / (uint32_t)a.G);
+    const int pos_hi = it.off + (int)((uint32_t)(it.row0 + min(wrow + 31, it.rows - 1)) / (uint32_t)a.G);
+    const int block_lo = it.off + (int)((uint32_t)it.row0 / (uint32_t)a.G);
+
+    auto step = [&](int key0, uint8_t* kt, uint8_t* vt, uint8_t* kn, uint8_t* vn) {
+        __builtin_amdgcn_s_waitcnt(0);  // this wave's loads of the tile are in LDS
+        // a tile that some row of the block sees in part: its V is looked over for infinities and NaN
+        // (with three terms every tile's K and V)
+        const bool part_seen = key0 + 63 > block_lo || key0 + 64 > it.k1;  // uniform over the block
+        uint32_t* const bad = bad_lds + 2 * ((key0 >> 6) & 1);
+        if (part_seen || TERMS > 1) {
+            uint32_t bk = 0, bv = 0;
+#pragma unroll
+            for (int n = 0; n < D / 32; n++) {
+                const int at = 16 * wave * L::ROWB + n * 1024 + 16 * lane;
+                const uint4 w = *reinterpret_cast<const uint4*>(vt + at);
+                bv |= t_nonfinite(w.x) | t_nonfinite(w.y) | t_nonfinite(w.z) | t_nonfinite(w.w);
+                if constexpr (TERMS > 1) {
+                    const uint4 y = *reinterpret_cast<const uint4*>(kt + at);
+                    bk |= t_nonfinite(y.x) | t_nonfinite(y.y) | t_nonfinite(y.z) | t_nonfinite(y.w);
+                }
+            }
+            if (bk) bad[0] = 1;
+            if (bv) bad[1] = 1;
+            __builtin_amdgcn_s_waitcnt(0xC07F);
+        }
+        t_barrier();
+        if (key0 + 64 < it.k1) src.load(key0 + 64 + 16 * wave, lane, kn + 16 * wave * L::ROWB, vn + 16 * wave * L::ROWB);
+        if (!has || key0 > pos_hi) return;
+        const bool bad_k = TERMS > 1 && bad[0] != 0, bad_v = (part_seen || TERMS > 1) && bad[1] != 0;
+        if (key0 + 63 > pos_lo || key0 + 64 > it.k1)
+            tile_step<D, TERMS, true>(s, kt, vt, key0, it.k1, c, bad_k, bad_v, lane);
+        else
+            tile_step<D, TERMS, false>(s, kt, vt, key0, it.k1, c, bad_k, bad_v, lane);
+    };
+    if (it.k0 < it.k1) {
+        src.load(it.k0 + 16 * wave, lane, kt0 + 16 * wave * L::ROWB, vt0 + 16 * wave * L::ROWB);
+        __syncthreads();  // bad_lds is cleared
+        for (int key0 = it.k0; key0 < it.k1; key0 += 128) {
+            step(key0, kt0, vt0, kt1, vt1);
+            if (key0 + 64 < it.k1) step(key0 + 64, kt1, vt1, kt0, vt0);
+        }
+    }
+    if (has) rows_store(s, a, it, h, wrow, lane);
+}
+
+}  // namespace oom

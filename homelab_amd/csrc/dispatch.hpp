@@ -294,6 +294,37 @@ inline int attn_pairs(int kv_len, int heads, int kv_heads, int d, size_t ws_byte
     return 8;
 }
 
+// ---- oom_attn_plan, oom_attn_prompt, oom_attn_chunk_paged (attn_plan.hip, attn_tile.hpp) -------
+
+constexpr int ATTN_ROWS = 128;        // packed rows (token, query head of a group) a tile
+constexpr int ATTN_KEYS = 64;         // keys a tile
+constexpr int ATTN_SPLIT_BLOCKS = 512;  // blocks that a batch's keys are split for: two a CU
+constexpr int ATTN_MAXB = 4096;       // sequences of a plan
+constexpr int ATTN_MAX_KEYS = 1 << 27;  // keys of a sequence
+
+// A plan in i32 words: ATTN_PLAN_HEAD words of counts, then the items, then the merges.
+constexpr int ATTN_PLAN_HEAD = 16;
+constexpr int ATTN_ITEM_WORDS = 8;
+constexpr int ATTN_PLAN_ITEMS = 0, ATTN_PLAN_MERGES = 1;  // head words: items, merges
+
+// The plan's bounds, from sizes that the host knows. Tiles of sequence b: ceil(n_b G / 128), so at
+// most T G / 128 + B in all. With W key tiles over them and splits of ks = ceil(W Hkv / 512),
+// the items number at most tiles + W / ks and the tiles that are split at all (more than ks
+// key tiles) at most W / ks <= ceil(512 / Hkv); their parts at most twice that.
+struct AttnPlanDims {
+    int64_t tiles, items, merges, part_rows, words;
+};
+inline AttnPlanDims attn_plan_dims(int64_t T, int64_t B, int heads, int kv_heads) {
+    AttnPlanDims p;
+    const int64_t rows = T * (heads / kv_heads), split = cdiv(ATTN_SPLIT_BLOCKS, kv_heads);
+    p.tiles = rows / ATTN_ROWS + B;
+    p.items = p.tiles + split;
+    p.merges = split;
+    p.part_rows = 2 * split * std::min<int64_t>(ATTN_ROWS, std::max<int64_t>(rows, 1));
+    p.words = ATTN_PLAN_HEAD + (p.items + p.merges) * ATTN_ITEM_WORDS;
+    return p;
+}
+
 // ---- oom_attn_decode_turbo (turbo.hip) ------------------------------------------------------
 
 // How a KV head's keys are dealt: blocks of `waves` waves, `blocks` of them a KV head. A wave's

@@ -394,6 +394,97 @@ int oom_attn_decode_turbo(const float* q, const uint8_t* k, const uint8_t* v, in
                           const float* levels, const uint8_t* mask, int heads, int kv_heads, int d, int kv_len,
                           float scale, float* out, void* ws, size_t ws_bytes, void* stream);
 
+/* ---- the prompt path: rotary positions, paged cache writes, prompt and chunk attention ----
+ * What fills the paged bf16 cache of oom_attn_decode_paged (k_pages and v_pages [n_pages,
+ * kv_heads, page_size, d]) and attends over it for a whole batch. A step over packed tokens:
+ *   oom_attn_plan once (positions, cache slots, the attention's work list), then per layer
+ *   oom_rope_append_paged and oom_attn_chunk_paged (or oom_attn_prompt over the step's own
+ *   rows, where every sequence starts at its first token).
+ * Tokens are packed: token rows of sequence b are [cu_q[b], cu_q[b + 1]) of T, rows at or past
+ * cu_q[B] belong to none and stay as they were. Strides are in elements, between tokens, so q, k
+ * and v may be slices of one fused projection's rows: multiples of 8, every base 16-byte
+ * aligned. None of these calls keeps state: a workspace needs no fill. */
+
+/* Which dims of a head form a pair, among its first rot_dim: (i, i + rot_dim / 2) or (2i, 2i + 1). */
+#define OOM_ROPE_HALF 0
+#define OOM_ROPE_INTERLEAVED 1
+/* Frequencies f_i = base^(-2 i / rot_dim): as they are, all divided by `factor`, or by parts
+ * (YaRN: pairs that turn at least beta_fast times over trained_len positions stay, those
+ * under beta_slow turns are divided by factor, a ramp between; cos and sin are multiplied by
+ * 0.1 ln(factor) + 1). */
+#define OOM_ROPE_PLAIN 0
+#define OOM_ROPE_LINEAR 1
+#define OOM_ROPE_YARN 2
+typedef struct OomRope {
+    int64_t rot_dim; /* even, at most 1024 */
+    int64_t scaling;
+    double base;        /* above 1 */
+    double factor;      /* LINEAR, YARN: at least 1 */
+    int64_t trained_len; /* YARN */
+    double beta_fast;
+    double beta_slow;
+} OomRope;
+/* The frequency table on the host (the device copy goes to the calls below): turns[i], i < rot_dim
+ * / 2, is f_i as a 64-bit fraction of a full turn, so that an angle of any 32-bit position is
+ * exact modulo a turn; n >= rot_dim / 2. *magnitude: the factor on cos and sin (1 but for YARN). */
+int oom_rope_table(const OomRope* rope, uint64_t* turns, size_t n, float* magnitude);
+/* Rotary positions of rows x [T, heads, d]: pair (u, w) of the first rot_dim dims -> magnitude *
+ * (u cos - w sin, u sin + w cos), angle positions[t] f_i (inverse 1: its negative, which for
+ * magnitude 1 takes a rotation back); dims from rot_dim on are copied. fp32 products, one
+ * rounding to out_dtype. d a multiple of 8 up to 1024. out may be x itself (same dtype and
+ * stride); otherwise the two must not overlap. The engine's rope_rotate_half
+ * (crates/oominf-cuda/kernels/attention.cu:136-183) and its interleaved form. */
+int oom_rope(const void* x, int x_dtype, int64_t x_stride, const int32_t* positions, const uint64_t* turns,
+             int rot_dim, int layout, float magnitude, int inverse, void* out, int out_dtype, int64_t out_stride,
+             int T, int heads, int d, void* stream);
+/* A step's rows into the cache: q_out = oom_rope(q), and k (rotated the same way) and v, rounded to
+ * bf16, at cache slot slots[t] (page slots[t] / page_size, slot slots[t] % page_size of every KV
+ * head). A slot outside [0, n_pages * page_size) writes nothing (its q_out is written). q
+ * [T, heads, d], k and v [T, kv_heads, d], all in x_dtype. q_out may be q. Two tokens of one
+ * call must not share a slot: the row would be either's. */
+int oom_rope_append_paged(const void* q, int64_t q_stride, const void* k, int64_t k_stride, const void* v,
+                          int64_t v_stride, int x_dtype, const int32_t* positions, const int64_t* slots,
+                          const uint64_t* turns, int rot_dim, int layout, float magnitude, void* q_out,
+                          int out_dtype, int64_t out_stride, uint16_t* k_pages, uint16_t* v_pages, int n_pages,
+                          int page_size, int T, int heads, int kv_heads, int d, void* stream);
+
+/* The plan of one step's batch of B sequences (at most 4096), made on the device from device
+ * lengths and used by the attention calls of every layer with the same T, B, heads, kv_heads
+ * and d: `plan` holds oom_attn_plan_size() i32 words, 16-byte aligned.
+ *   cu_q i32 [B + 1], rising from 0 or more to at most T;
+ *   kv_lens i32 [B]: keys in the cache after this step's tokens are written (new token i of n is
+ *   at position kv_len - n + i; a negative position sees nothing), page_table i32 [B, max_pages];
+ *   both null for prompts (oom_attn_prompt), whose keys are their own tokens.
+ * A length past the table's pages is taken as theirs. positions i32 [T] and slots i64 [T], each
+ * may be null, get each token's position and cache slot (0 and -1 for a token of no
+ * sequence; slot -1 where the table's page is not in [0, n_pages)); slots need a page_table. */
+size_t oom_attn_plan_size(int T, int B, int heads, int kv_heads, int d);
+int oom_attn_plan(const int32_t* cu_q, const int32_t* kv_lens, const int32_t* page_table, int max_pages,
+                  int n_pages, int page_size, int T, int B, int heads, int kv_heads, int d, int32_t* positions,
+                  int64_t* slots, int32_t* plan, void* stream);
+/* Causal attention of packed prompts: out[t, h, :] = sum_j softmax_j(q[t, h] . k[j, g] * scale)
+ * v[j, g] over the tokens j of t's sequence up to t, g = h / (heads / kv_heads). q [T, heads, d] in
+ * q_dtype; k and v bf16 [T, kv_heads, d]; out [T, heads, d] in out_dtype. d 64, 128 or 256; any
+ * number of query heads a KV head; scale positive. plan: oom_attn_plan's with null kv_lens.
+ * Keys that a token does not see have no part in its row, whatever they hold. fp32 on either
+ * side: fp32 products, sums and exponentials (three exact bf16 terms on the matrix cores);
+ * bf16 on both: the weights p enter the second product rounded to bf16, sums in fp32.
+ * Replaces Attention::attention at prefill (crates/oominf-core/src/backend.rs:545-568;
+ * crates/oominf-cuda/src/attention.rs:265-346) over packed rows. */
+int oom_attn_prompt(const void* q, int q_dtype, int64_t q_stride, const uint16_t* k, int64_t k_stride,
+                    const uint16_t* v, int64_t v_stride, const int32_t* plan, int T, int B, int heads, int kv_heads,
+                    int d, float scale, void* out, int out_dtype, int64_t out_stride, void* stream);
+/* Attention of a step's new tokens, one or many a sequence, over the paged cache that already
+ * holds their rows: the token at position p sees the keys 0 .. p of its sequence; a token that
+ * sees none gets zeros. max_q bounds the new tokens of any sequence (1: a decode step). plan:
+ * oom_attn_plan's with kv_lens and page_table. A page index outside [0, n_pages) reads zeros.
+ * Types, products and heads as oom_attn_prompt, page_size a multiple of 16. */
+size_t oom_attn_chunk_paged_workspace_size(int T, int B, int heads, int kv_heads, int d);
+int oom_attn_chunk_paged(const void* q, int q_dtype, int64_t q_stride, const uint16_t* k_pages,
+                         const uint16_t* v_pages, const int32_t* page_table, int max_pages, int n_pages,
+                         int page_size, const int32_t* plan, int T, int B, int max_q, int heads, int kv_heads, int d,
+                         float scale, void* out, int out_dtype, int64_t out_stride, void* ws, size_t ws_bytes,
+                         void* stream);
 
 /* ---- copies beside compute (expert offload) ----
  * The Transfer trait (crates/oominf-core/src/backend.rs:945-1018; CUDA form

@@ -93,6 +93,22 @@ struct TileLay {
     static __device__ __forceinline__ int vx(int row) { return D == 64 ? ((row >> 1) & 1) * 2 : (row & 3) * 4; }
 };
 
+// 16 bytes a lane straight into LDS: lane l's land at lds + 16 l (lds uniform). In assembly, so that
+// the compiler does not wait for these loads before LDS reads of another stage: the kernel's own
+// waits and barriers order them. The address is a uniform base plus a 32-bit offset a lane.
+__device__ __forceinline__ void t_load_lds(const void* base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base)
+                 : "memory", "m0");
+}
+__device__ __forceinline__ void t_load_lds(const void* at, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at)
+                 : "memory", "m0");
+}
+// This wave's loads into LDS, and its LDS reads and writes, are done.
+__device__ __forceinline__ void t_wait_loads() {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+}
+
 // Loads of one 64-key tile: wave w of 4 takes rows 16 w .. 16 w + 15 of K and of V, which lie in
 // one page.
 template <int D, bool PAGED>
@@ -102,81 +118,65 @@ struct TileSrc {
     const uint16_t *k, *v;
     int64_t ks, vs;  // elements between rows
     const int32_t* table;
-    int n_pages, p16, head, k1;
+    int n_pages, p16, k1;
     int64_t page_elems;
-    int ko[NI], vo;  // byte offsets of this lane from the wave's first row
+    uint32_t ko[NI], vo[NI];  // byte offsets of this lane from the wave's first row
 
     __device__ __forceinline__ void init(const TileArgs& a, const AttnItem& it, int h, int lane) {
         k1 = it.k1;
         if constexpr (PAGED) {
             ks = vs = D;
-            k = a.k;
-            v = a.v;
             table = a.table + (size_t)it.seq * a.max_pages;
             n_pages = a.n_pages;
             p16 = a.page_size / 16;
-            head = h;
             page_elems = (int64_t)a.page_size * a.Hkv * D;
+            k = a.k + (int64_t)h * a.page_size * D;
+            v = a.v + (int64_t)h * a.page_size * D;
         } else {
             ks = a.k_stride;
             vs = a.v_stride;
             k = a.k + (int64_t)it.q0 * ks + h * D;
             v = a.v + (int64_t)it.q0 * vs + h * D;
         }
-        const int r = lane / L::C, c = lane % L::C;
 #pragma unroll
-        for (int n = 0; n < NI; n++) ko[n] = (int)((n * L::RPI + r) * ks * 2) + 16 * (c ^ L::kx(n * L::RPI + r));
-        vo = (int)(r * vs * 2) + 16 * (c ^ L::vx(r));
-        static_assert(L::RPI % 4 == 0 || L::RPI == 2, "V's permutation per instruction");
+        for (int n = 0; n < NI; n++) {
+            const int r = n * L::RPI + lane / L::C, c = lane % L::C;
+            ko[n] = (uint32_t)(r * ks * 2) + 16 * (c ^ L::kx(r));
+            vo[n] = (uint32_t)(r * vs * 2) + 16 * (c ^ L::vx(r));
+        }
     }
 
-    // The wave's 16 rows from key `key` (a multiple of 16) on into its places kt and vt (the
-    // tiles + 16 w rows).
-    __device__ __forceinline__ void load(int key, int lane, uint8_t* kt, uint8_t* vt) const {
-        const uint16_t *kb = nullptr, *vb = nullptr;
+    // The wave's 16 rows from key `key` (a multiple of 16) on into its places kt and vt (LDS byte
+    // addresses of its first row in the K and the V tile).
+    __device__ __forceinline__ void load(int key, int lane, uint32_t kt, uint32_t vt) const {
+        int64_t kat = 0, vat = 0;
         bool ok = key < k1;
         if constexpr (PAGED) {
             if (ok) {
                 const uint32_t sub = (uint32_t)key / 16, pi = sub / (uint32_t)p16, si = sub - pi * p16;
                 const int page = table[pi];
                 ok = page >= 0 && page < n_pages;
-                const int64_t at = (ok ? page : 0) * page_elems + ((int64_t)head * p16 + si) * 16 * D;
-                kb = k + at;
-                vb = v + at;
+                kat = vat = (ok ? page : 0) * page_elems + (int64_t)si * 16 * D;
             }
         } else {
-            kb = k + key * ks;
-            vb = v + key * vs;
+            kat = key * ks;
+            vat = key * vs;
         }
+        const uint16_t *kb = k + kat, *vb = v + vat;
         if (ok && key + 16 <= k1) {  // uniform
 #pragma unroll
-            for (int n = 0; n < NI; n++)
-                __builtin_amdgcn_global_load_lds((t_glb_t)((const uint8_t*)kb + ko[n]),
-                                                 (t_lds_t)(kt + n * 1024), 16, 0, 0);
+            for (int n = 0; n < NI; n++) t_load_lds(kb, ko[n], kt + n * 1024);
 #pragma unroll
-            for (int n = 0; n < NI; n++)
-                __builtin_amdgcn_global_load_lds((t_glb_t)((const uint8_t*)vb + v_off(n, lane)),
-                                                 (t_lds_t)(vt + n * 1024), 16, 0, 0);
+            for (int n = 0; n < NI; n++) t_load_lds(vb, vo[n], vt + n * 1024);
             return;
         }
-        const int r = lane / L::C, c = lane % L::C;
-        const uint8_t* z = (const uint8_t*)t_zero_row + 16 * c;
+        const uint8_t* z = (const uint8_t*)t_zero_row + 16 * (lane % L::C);
 #pragma unroll
         for (int n = 0; n < NI; n++) {
-            const bool in = ok && key + n * L::RPI + r < k1;
-            __builtin_amdgcn_global_load_lds((t_glb_t)(in ? (const uint8_t*)kb + ko[n] : z), (t_lds_t)(kt + n * 1024),
-                                             16, 0, 0);
-            __builtin_amdgcn_global_load_lds((t_glb_t)(in ? (const uint8_t*)vb + v_off(n, lane) : z),
-                                             (t_lds_t)(vt + n * 1024), 16, 0, 0);
+            const bool in = ok && key + n * L::RPI + lane / L::C < k1;
+            t_load_lds(in ? (const uint8_t*)kb + ko[n] : z, kt + n * 1024);
+            t_load_lds(in ? (const uint8_t*)vb + vo[n] : z, vt + n * 1024);
         }
-    }
-
-    __device__ __forceinline__ int64_t v_off(int n, int lane) const {
-        // rows of instruction n are n RPI + lane / C: with RPI a multiple of 4 the permutation does
-        // not depend on n; with two rows an instruction it alternates
-        if constexpr (L::RPI % 4 == 0) return vo + (int64_t)n * L::RPI * vs * 2;
-        const int r = lane / L::C, c = lane % L::C;
-        return (n * L::RPI + r) * vs * 2 + 16 * (c ^ L::vx(n * L::RPI + r));
     }
 };
 
@@ -191,7 +191,7 @@ __device__ __forceinline__ uint32_t t_finite(uint32_t w) {
 
 // TERMS 1: bf16 queries and outputs: the products take Q as it is and P rounded to bf16 (its
 // relative error, at most 2^-8 a key and averaged over the keys, is of the size of the
-// output's own rounding). TERMS 3: fp32 on either side: Q and P enter as three exact bf16
+// output's own rounding; the sum l is that of the rounded p). TERMS 3: fp32 on either side: Q and P enter as three exact bf16
 // terms each (hi + mid + lo), so products are exact and only fp32 sums round.
 template <int D, int TERMS>
 struct RowState {
@@ -268,9 +268,8 @@ __device__ __forceinline__ void tile_step(RowState<D, TERMS>& s, const uint8_t* 
 #pragma unroll
     for (int n = 0; n < 2; n++) {
 #pragma unroll
-        for (int i = 0; i < 16; i++) sc[n][i] = 0.0f;
-#pragma unroll
         for (int st = 0; st < D / 16; st++) {
+            if (st == 0) sc[n] = tf32x16{};
             const uint4 kv = *reinterpret_cast<const uint4*>(krow + 32 * n * L::ROWB + 16 * ((2 * st + half) ^ kx));
             const tbf16x8 ka = __builtin_bit_cast(tbf16x8, kv);
             if constexpr (TERMS > 1) {
@@ -310,24 +309,30 @@ __device__ __forceinline__ void tile_step(RowState<D, TERMS>& s, const uint8_t* 
 #pragma unroll
             for (int i = 0; i < 16; i++) s.o[d][i] *= f;
     }
-    const float m0 = s.m == -INFINITY ? 0.0f : s.m, mb = m0 * c;
+    float m0 = s.m == -INFINITY ? 0.0f : s.m;
+    if (c > 1.0f) {  // uniform
+#pragma unroll
+        for (int n = 0; n < 2; n++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) sc[n][i] -= m0;
+        m0 = 0.0f;
+    }
+    const float mb = m0 * c;
     // ---- p, its sum, and the products, 16 keys at a time ----
+    const tbf16x2 ones = __builtin_bit_cast(tbf16x2, 0x3f803f80u);
+    float sum = 0.0f;
     const int grp = lane >> 4, r4 = (lane & 15) >> 2;
     const uint8_t* vrow = vt + (4 * half + r4) * L::ROWB + 8 * (lane & 1);
     const int vc = 2 * (grp & 1) + ((lane & 3) >> 1), vx = L::vx(4 * half + r4);
 #pragma unroll
     for (int n = 0; n < 2; n++) {
-        float p[16], sum = 0.0f;
-        if (c <= 1.0f) {  // uniform
+        float p[16];
 #pragma unroll
-            for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[n][i], c, -mb));
-        } else {
+        for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[n][i], c, -mb));
+        if constexpr (TERMS > 1) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f((sc[n][i] - m0) * c);
+            for (int i = 0; i < 16; i++) sum += p[i];
         }
-#pragma unroll
-        for (int i = 0; i < 16; i++) sum += p[i];
-        s.l += sum;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             tbf16x8 pb[TERMS];
@@ -338,6 +343,7 @@ __device__ __forceinline__ void tile_step(RowState<D, TERMS>& s, const uint8_t* 
                 for (int e = 0; e < 4; e++) {
                     float &x = p[8 * u + 2 * e], &y = p[8 * u + 2 * e + 1];
                     w[e] = t_pack(x, y);
+                    if (TERMS == 1) sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(tbf16x2, w[e]), ones, sum, false);
                     if (t + 1 < TERMS) {
                         x -= __uint_as_float(w[e] << 16);
                         y -= __uint_as_float(w[e] & 0xffff0000u);
@@ -360,6 +366,7 @@ __device__ __forceinline__ void tile_step(RowState<D, TERMS>& s, const uint8_t* 
             }
         }
     }
+    s.l += sum;
     if constexpr (MASKED) {
         if (bad_v) {  // uniform; rare: infinities and NaN of V reach the rows that see their key
             const int last = min(s.pos, k1 - 1) - key0;
@@ -430,10 +437,8 @@ __device__ __forceinline__ void rows_store(RowState<D, TERMS>& s, const TileArgs
 template <int D, int TERMS, bool PAGED>
 __global__ void __launch_bounds__(256, (D <= 128 && TERMS == 1) ? 2 : 1) attn_tile_kernel(TileArgs a) {
     typedef TileLay<D> L;
-    // each stage its own LDS object, so the compiler's waits for direct-to-LDS loads cover only the
-    // loads into the buffer a read touches
-    __shared__ __align__(16) uint8_t kt0[L::BYTES], vt0[L::BYTES], kt1[L::BYTES], vt1[L::BYTES];
-    __shared__ uint32_t bad_lds[4];  // per stage: K, V hold infinities or NaN
+    __shared__ __align__(16) uint8_t tiles[4 * L::BYTES];  // stage 0: K, V; stage 1: K, V
+    __shared__ uint32_t bad_lds[4];                        // per stage: K, V hold infinities or NaN
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = (int)(blockIdx.x % (uint32_t)a.Hkv), item = (int)(blockIdx.x / (uint32_t)a.Hkv);
@@ -445,51 +450,59 @@ __global__ void __launch_bounds__(256, (D <= 128 && TERMS == 1) ? 2 : 1) attn_ti
     TileSrc<D, PAGED> src;
     src.init(a, it, h, lane);
     if (threadIdx.x < 4) bad_lds[threadIdx.x] = 0;
+    const uint32_t mine = (uint32_t)(uintptr_t)(t_lds_t)tiles + 16 * wave * L::ROWB;  // LDS address of the wave's rows
+    const bool any = it.k0 < it.k1;
+    if (any) src.load(it.k0 + 16 * wave, lane, mine, mine + L::BYTES);
     RowState<D, TERMS> s;
     rows_init(s, a, it, h, wrow, lane);
-    // positions of the wave's first and last row
-    const int pos_lo = it.off + (int)((uint32_t)(it.row0 + min(wrow, it.rows - 1)) / (uint32_t)a.G);
+    __syncthreads();  // bad_lds is cleared
+    // the wave's last position; the tiles that every row of the block sees whole come first
     const int pos_hi = it.off + (int)((uint32_t)(it.row0 + min(wrow + 31, it.rows - 1)) / (uint32_t)a.G);
     const int block_lo = it.off + (int)((uint32_t)it.row0 / (uint32_t)a.G);
+    const int whole = it.k0 + (max(0, min(it.k1, block_lo + 1) - it.k0) & ~63);
+    int key0 = it.k0;
+    uint32_t stage = 0;
 
-    auto step = [&](int key0, uint8_t* kt, uint8_t* vt, uint8_t* kn, uint8_t* vn) {
-        __builtin_amdgcn_s_waitcnt(0);  // this wave's loads of the tile are in LDS
-        // a tile that some row of the block sees in part: its V is looked over for infinities and NaN
-        // (with three terms every tile's K and V)
-        const bool part_seen = key0 + 63 > block_lo || key0 + 64 > it.k1;  // uniform over the block
-        uint32_t* const bad = bad_lds + 2 * ((key0 >> 6) & 1);
-        if (part_seen || TERMS > 1) {
-            uint32_t bk = 0, bv = 0;
-#pragma unroll
-            for (int n = 0; n < D / 32; n++) {
-                const int at = 16 * wave * L::ROWB + n * 1024 + 16 * lane;
-                const uint4 w = *reinterpret_cast<const uint4*>(vt + at);
-                bv |= t_nonfinite(w.x) | t_nonfinite(w.y) | t_nonfinite(w.z) | t_nonfinite(w.w);
-                if constexpr (TERMS > 1) {
-                    const uint4 y = *reinterpret_cast<const uint4*>(kt + at);
-                    bk |= t_nonfinite(y.x) | t_nonfinite(y.y) | t_nonfinite(y.z) | t_nonfinite(y.w);
-                }
-            }
-            if (bk) bad[0] = 1;
-            if (bv) bad[1] = 1;
-            __builtin_amdgcn_s_waitcnt(0xC07F);
+    const auto next = [&]() {
+        if (key0 + 64 < it.k1) {
+            const uint32_t to = mine + (stage ^ (2 * L::BYTES));
+            src.load(key0 + 64 + 16 * wave, lane, to, to + L::BYTES);
         }
-        t_barrier();
-        if (key0 + 64 < it.k1) src.load(key0 + 64 + 16 * wave, lane, kn + 16 * wave * L::ROWB, vn + 16 * wave * L::ROWB);
-        if (!has || key0 > pos_hi) return;
-        const bool bad_k = TERMS > 1 && bad[0] != 0, bad_v = (part_seen || TERMS > 1) && bad[1] != 0;
-        if (key0 + 63 > pos_lo || key0 + 64 > it.k1)
-            tile_step<D, TERMS, true>(s, kt, vt, key0, it.k1, c, bad_k, bad_v, lane);
-        else
-            tile_step<D, TERMS, false>(s, kt, vt, key0, it.k1, c, bad_k, bad_v, lane);
     };
-    if (it.k0 < it.k1) {
-        src.load(it.k0 + 16 * wave, lane, kt0 + 16 * wave * L::ROWB, vt0 + 16 * wave * L::ROWB);
-        __syncthreads();  // bad_lds is cleared
-        for (int key0 = it.k0; key0 < it.k1; key0 += 128) {
-            step(key0, kt0, vt0, kt1, vt1);
-            if (key0 + 64 < it.k1) step(key0 + 64, kt1, vt1, kt0, vt0);
+    // K's (three terms) and V's infinities and NaN in the wave's part of the tile
+    const auto look = [&]() {
+        uint32_t bk = 0, bv = 0;
+#pragma unroll
+        for (int n = 0; n < D / 32; n++) {
+            const uint8_t* at = tiles + stage + 16 * wave * L::ROWB + n * 1024 + 16 * lane;
+            const uint4 w = *reinterpret_cast<const uint4*>(at + L::BYTES);
+            bv |= t_nonfinite(w.x) | t_nonfinite(w.y) | t_nonfinite(w.z) | t_nonfinite(w.w);
+            if constexpr (TERMS > 1) {
+                const uint4 y = *reinterpret_cast<const uint4*>(at);
+                bk |= t_nonfinite(y.x) | t_nonfinite(y.y) | t_nonfinite(y.z) | t_nonfinite(y.w);
+            }
         }
+        uint32_t* const bad = bad_lds + (stage ? 2 : 0);
+        if (bk) bad[0] = 1;
+        if (bv) bad[1] = 1;
+        __builtin_amdgcn_s_waitcnt(0xC07F);
+    };
+    for (; key0 < whole; key0 += 64, stage ^= 2 * L::BYTES) {
+        t_wait_loads();
+        if constexpr (TERMS > 1) look();
+        t_barrier();
+        next();
+        const bool bad_k = TERMS > 1 && bad_lds[stage ? 2 : 0] != 0, bad_v = TERMS > 1 && bad_lds[stage ? 3 : 1] != 0;
+        if (has) tile_step<D, TERMS, false>(s, tiles + stage, tiles + stage + L::BYTES, key0, it.k1, c, bad_k, bad_v, lane);
+    }
+    for (; key0 < it.k1; key0 += 64, stage ^= 2 * L::BYTES) {
+        t_wait_loads();
+        look();
+        t_barrier();
+        next();
+        const bool bad_k = TERMS > 1 && bad_lds[stage ? 2 : 0] != 0, bad_v = bad_lds[stage ? 3 : 1] != 0;
+        if (has && key0 <= pos_hi)
+            tile_step<D, TERMS, true>(s, tiles + stage, tiles + stage + L::BYTES, key0, it.k1, c, bad_k, bad_v, lane);
     }
     if (has) rows_store(s, a, it, h, wrow, lane);
 }

@@ -104,9 +104,13 @@ __device__ __forceinline__ void t_load_lds(const void* at, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(lds), "v"(at)
                  : "memory", "m0");
 }
-// This wave's loads into LDS, and its LDS reads and writes, are done.
+// This wave's loads into LDS, and its LDS reads and writes, are done. A builtin, which the compiler's
+// own accounting sees: past it, no load of its own is outstanding, and it places no wait for one
+// inside the tile loop, where it would wait for the loads into LDS too.
 __device__ __forceinline__ void t_wait_loads() {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0);
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
 // Loads of one 64-key tile: wave w of 4 takes rows 16 w .. 16 w + 15 of K and of V, which lie in

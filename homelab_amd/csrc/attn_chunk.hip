@@ -50,12 +50,11 @@ __global__ void __launch_bounds__(256) attn_rows_merge_kernel(TileArgs a, int64_
 
 template <int D>
 static int launch_chunk(const TileArgs& a, const AttnPlanDims& p, int64_t rows, bool exact, hipStream_t st) {
-    const dim3 grid((uint32_t)(p.items * a.Hkv)), block(256);
-    if (exact) hipLaunchKernelGGL((attn_tile_kernel<D, 3, true>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((attn_tile_kernel<D, 1, true>), grid, block, 0, st, a);
+    const dim3 grid((uint32_t)(p.items * a.Hkv));
+    launch_tiles<D, true>(a, grid, exact, st);
     if (int rc = launched("oom_attn_chunk_paged")) return rc;
     const dim3 mgrid((uint32_t)(p.merges * a.Hkv), (uint32_t)cdiv(std::min<int64_t>(rows, ATTN_ROWS), 16));
-    hipLaunchKernelGGL((attn_rows_merge_kernel<D>), mgrid, block, 0, st, a, p.items);
+    hipLaunchKernelGGL((attn_rows_merge_kernel<D>), mgrid, dim3(256), 0, st, a, p.items);
     return launched("oom_attn_chunk_paged");
 }
 

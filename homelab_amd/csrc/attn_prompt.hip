@@ -8,9 +8,8 @@ namespace oom {
 
 template <int D>
 static int launch_prompt(const TileArgs& a, int64_t items, bool exact, hipStream_t st) {
-    const dim3 grid((uint32_t)(items * a.Hkv)), block(256);
-    if (exact) hipLaunchKernelGGL((attn_tile_kernel<D, 3, false>), grid, block, 0, st, a);
-    else hipLaunchKernelGGL((attn_tile_kernel<D, 1, false>), grid, block, 0, st, a);
+    const dim3 grid((uint32_t)(items * a.Hkv));
+    launch_tiles<D, false>(a, grid, exact, st);
     return launched("oom_attn_prompt");
 }
 

@@ -19,6 +19,8 @@
 //    then the older maximum keeps every p below 2^8, which fp32 sums hold as well.
 #pragma once
 
+#include <type_traits>
+
 #include "common.hpp"
 
 namespace oom {
@@ -113,12 +115,12 @@ __device__ __forceinline__ void t_wait_loads() {
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
-// Loads of one 64-key tile: wave w of 4 takes rows 16 w .. 16 w + 15 of K and of V, which lie in
-// one page.
-template <int D, bool PAGED>
+// Loads of one 64-key tile: wave w of NW takes 64 / NW rows of K and of V, which lie in one page.
+template <int D, int NW, bool PAGED>
 struct TileSrc {
     typedef TileLay<D> L;
-    static constexpr int NI = 16 / L::RPI;  // instructions a wave
+    static constexpr int WR = 64 / NW, NI = WR / L::RPI;  // rows and instructions a wave
+    static_assert(NI >= 1 && WR <= 16 && 16 % WR == 0, "whole instructions, one 16-key run");
     const uint16_t *k, *v;
     int64_t ks, vs;  // elements between rows
     const int32_t* table;
@@ -126,7 +128,7 @@ struct TileSrc {
     int64_t page_elems;
     uint32_t ko[NI], vo[NI];  // byte offsets of this lane from the wave's first row
 
-    __device__ __forceinline__ void init(const TileArgs& a, const AttnItem& it, int h, int lane) {
+    __device__ __forceinline__ void init(const TileArgs& a, const AttnItem& it, int h, int lane, int wave) {
         k1 = it.k1;
         if constexpr (PAGED) {
             ks = vs = D;
@@ -145,12 +147,12 @@ struct TileSrc {
 #pragma unroll
         for (int n = 0; n < NI; n++) {
             const int r = n * L::RPI + lane / L::C, c = lane % L::C;
-            ko[n] = (uint32_t)(r * ks * 2) + 16 * (c ^ L::kx(r));
-            vo[n] = (uint32_t)(r * vs * 2) + 16 * (c ^ L::vx(r));
+            ko[n] = (uint32_t)(r * ks * 2) + 16 * (c ^ L::kx(WR * wave + r));
+            vo[n] = (uint32_t)(r * vs * 2) + 16 * (c ^ L::vx(WR * wave + r));
         }
     }
 
-    // The wave's 16 rows from key `key` (a multiple of 16) on into its places kt and vt (LDS byte
+    // The wave's rows from key `key` (a multiple of 64 / NW) on into its places kt and vt (LDS byte
     // addresses of its first row in the K and the V tile).
     __device__ __forceinline__ void load(int key, int lane, uint32_t kt, uint32_t vt) const {
         int64_t kat = 0, vat = 0;
@@ -160,14 +162,14 @@ struct TileSrc {
                 const uint32_t sub = (uint32_t)key / 16, pi = sub / (uint32_t)p16, si = sub - pi * p16;
                 const int page = table[pi];
                 ok = page >= 0 && page < n_pages;
-                kat = vat = (ok ? page : 0) * page_elems + (int64_t)si * 16 * D;
+                kat = vat = (ok ? page : 0) * page_elems + (int64_t)(si * 16 + key % 16) * D;
             }
         } else {
             kat = key * ks;
             vat = key * vs;
         }
         const uint16_t *kb = k + kat, *vb = v + vat;
-        if (ok && key + 16 <= k1) {  // uniform
+        if (ok && key + WR <= k1) {  // uniform
 #pragma unroll
             for (int n = 0; n < NI; n++) t_load_lds(kb, ko[n], kt + n * 1024);
 #pragma unroll
@@ -193,38 +195,69 @@ __device__ __forceinline__ uint32_t t_finite(uint32_t w) {
     return w & ~m;
 }
 
+typedef float tf32x4 __attribute__((ext_vector_type(4)));
+
+// The matrix instruction of M rows: S^T tiles of M keys x M rows over 512 / M dims, O^T tiles of M
+// dims x M rows over 512 / M keys. Lane l holds row l % M, and of a result's keys or dims the
+// four 4 (l / M) .. + 3 of each run of 256 / M: element i of a result is its key (dim)
+// (256 / M) (i / 4) + 4 (l / M) + i % 4.
+template <int M>
+struct Mx;
+template <>
+struct Mx<32> {
+    typedef tf32x16 acc;
+    static __device__ __forceinline__ acc mul(tbf16x8 a, tbf16x8 b, acc c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+    }
+};
+template <>
+struct Mx<16> {
+    typedef tf32x4 acc;
+    static __device__ __forceinline__ acc mul(tbf16x8 a, tbf16x8 b, acc c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+
 // TERMS 1: bf16 queries and outputs: the products take Q as it is and P rounded to bf16 (its
 // relative error, at most 2^-8 a key and averaged over the keys, is of the size of the
-// output's own rounding; the sum l is that of the rounded p). TERMS 3: fp32 on either side: Q and P enter as three exact bf16
-// terms each (hi + mid + lo), so products are exact and only fp32 sums round.
-template <int D, int TERMS>
+// output's own rounding; the sum l is that of the rounded p). TERMS 3: fp32 on either side: Q
+// and P enter as three exact bf16 terms each (hi + mid + lo), so products are exact and only
+// fp32 sums round.
+template <int D, int TERMS, int M>
 struct RowState {
-    tbf16x8 q[TERMS][D / 16];
-    tf32x16 o[D / 32];
+    static constexpr int KD = 512 / M;    // dims (keys) a product sums over
+    static constexpr int E = M * M / 64;  // elements of a result a lane
+    static constexpr int NS = 64 / M;     // results a tile of scores
+    typedef typename Mx<M>::acc acc;
+    tbf16x8 q[TERMS][D / KD];
+    acc o[D / M];
+    acc sc[NS];  // scores of the present tile
     float m, l;
     int pos;    // the last key this lane's row sees
     bool live;  // the lane has a row
 };
+// The key of element i of score result n, without the lane's 4 (l / M).
+template <int M>
+constexpr int score_key(int n, int i) { return M * n + (256 / M) * (i / 4) + i % 4; }
 
-template <int D, int TERMS>
-__device__ __forceinline__ void rows_init(RowState<D, TERMS>& s, const TileArgs& a, const AttnItem& it, int h, int wrow,
+template <int D, int TERMS, int M>
+__device__ __forceinline__ void rows_init(RowState<D, TERMS, M>& s, const TileArgs& a, const AttnItem& it, int h, int wrow,
                                           int lane) {
-    const int r = wrow + (lane & 31), half = lane >> 5;
+    const int r = wrow + lane % M, part = lane / M;
     s.live = r < it.rows;
     const uint32_t row = (uint32_t)(it.row0 + (s.live ? r : 0)), tok = row / (uint32_t)a.G, g = row - tok * a.G;
     s.pos = it.off + (int)tok;
     s.m = -INFINITY;
     s.l = 0.0f;
 #pragma unroll
-    for (int d = 0; d < D / 32; d++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) s.o[d][i] = 0.0f;
-    const int64_t at = (int64_t)(it.q0 + (int)tok) * a.q_stride + (int64_t)(h * a.G + (int)g) * D + 8 * half;
+    for (int d = 0; d < D / M; d++) s.o[d] = typename Mx<M>::acc{};
+    constexpr int KD = 512 / M;
+    const int64_t at = (int64_t)(it.q0 + (int)tok) * a.q_stride + (int64_t)(h * a.G + (int)g) * D + 8 * part;
     if (a.q_dtype == OOM_BF16) {
         const uint16_t* p = reinterpret_cast<const uint16_t*>(a.q) + at;
 #pragma unroll
-        for (int c = 0; c < D / 16; c++) {
-            const uint4 v = *reinterpret_cast<const uint4*>(p + 16 * c);
+        for (int c = 0; c < D / KD; c++) {
+            const uint4 v = *reinterpret_cast<const uint4*>(p + KD * c);
             s.q[0][c] = __builtin_bit_cast(tbf16x8, v);
             if constexpr (TERMS == 3)
                 s.q[1][c] = s.q[2][c] = __builtin_bit_cast(tbf16x8, make_uint4(0, 0, 0, 0));
@@ -232,9 +265,9 @@ __device__ __forceinline__ void rows_init(RowState<D, TERMS>& s, const TileArgs&
     } else if constexpr (TERMS == 3) {
         const float* p = reinterpret_cast<const float*>(a.q) + at;
 #pragma unroll
-        for (int c = 0; c < D / 16; c++) {
-            const float4 v0 = *reinterpret_cast<const float4*>(p + 16 * c);
-            const float4 v1 = *reinterpret_cast<const float4*>(p + 16 * c + 4);
+        for (int c = 0; c < D / KD; c++) {
+            const float4 v0 = *reinterpret_cast<const float4*>(p + KD * c);
+            const float4 v1 = *reinterpret_cast<const float4*>(p + KD * c + 4);
             float f[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
 #pragma unroll
             for (int t = 0; t < 3; t++) {
@@ -256,177 +289,199 @@ __device__ __forceinline__ tbf16x8 t_finite8(tbf16x8 v) {
     return __builtin_bit_cast(tbf16x8, make_uint4(t_finite(w.x), t_finite(w.y), t_finite(w.z), t_finite(w.w)));
 }
 
-// One 64-key tile from LDS. MASKED: some key of the tile is hidden from some row (a later
-// position, or past the item's keys), and V may hold infinities or NaN there (bad_v): those are
-// taken out of the product and added to the rows that see them. With three terms, an infinity of
-// K (bad_k) or V meets the first alone: the others may be zero or of the other sign.
-template <int D, int TERMS, bool MASKED>
-__device__ __forceinline__ void tile_step(RowState<D, TERMS>& s, const uint8_t* kt, const uint8_t* vt, int key0, int k1,
-                                          float c, bool bad_k, bool bad_v, int lane) {
+// One 64-key tile from LDS. MASKED: some key of the tile is hidden from some row, by a later position
+// or past the item's keys (last: the last one that the lane's row sees). BAD_K, with three terms: K
+// holds infinities or NaN, which meet the first term alone; the others may be zero or of the
+// other sign. V holds none (the kernel takes them out).
+template <int D, int TERMS, int M, bool MASKED, bool BAD_K>
+__device__ __forceinline__ void tile_scores(RowState<D, TERMS, M>& s, const uint8_t* kt, int last, int lane) {
     typedef TileLay<D> L;
-    const int half = lane >> 5;
-    // ---- scores: 32 keys at a time; lane: key 32 n + 8 (i / 4) + 4 half + i % 4 of row l % 32 ----
-    tf32x16 sc[2];
-    const uint8_t* krow = kt + (lane & 31) * L::ROWB;
-    const int kx = L::kx(lane & 31);
+    typedef RowState<D, TERMS, M> S;
+    const int part = lane / M;
+    const uint8_t* krow = kt + (lane % M) * L::ROWB;
+    const int kx = L::kx(lane % M);  // rows M apart have the same
 #pragma unroll
-    for (int n = 0; n < 2; n++) {
+    for (int n = 0; n < S::NS; n++) {
+        s.sc[n] = typename S::acc{};
 #pragma unroll
-        for (int st = 0; st < D / 16; st++) {
-            if (st == 0) sc[n] = tf32x16{};
-            const uint4 kv = *reinterpret_cast<const uint4*>(krow + 32 * n * L::ROWB + 16 * ((2 * st + half) ^ kx));
+        for (int st = 0; st < D / S::KD; st++) {
+            const int chunk = (S::KD / 8 * st + part) ^ kx;
+            const uint4 kv = *reinterpret_cast<const uint4*>(krow + M * n * L::ROWB + 16 * chunk);
             const tbf16x8 ka = __builtin_bit_cast(tbf16x8, kv);
             if constexpr (TERMS > 1) {
-                const tbf16x8 kf = bad_k ? t_finite8(ka) : ka;
+                const tbf16x8 kf = BAD_K ? t_finite8(ka) : ka;
 #pragma unroll
-                for (int t = TERMS - 1; t > 0; t--)
-                    sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf, s.q[t][st], sc[n], 0, 0, 0);
+                for (int t = TERMS - 1; t > 0; t--) s.sc[n] = Mx<M>::mul(kf, s.q[t][st], s.sc[n]);
             }
-            sc[n] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(ka, s.q[0][st], sc[n], 0, 0, 0);
+            s.sc[n] = Mx<M>::mul(ka, s.q[0][st], s.sc[n]);
         }
     }
     if constexpr (MASKED) {
-        const int last = min(s.pos, k1 - 1) - key0;
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+        for (int n = 0; n < S::NS; n++)
 #pragma unroll
-            for (int i = 0; i < 16; i++)
-                if (32 * n + 8 * (i / 4) + 4 * half + i % 4 > last) sc[n][i] = -INFINITY;
+            for (int i = 0; i < S::E; i++)
+                if (score_key<M>(n, i) + 4 * part > last) s.sc[n][i] = -INFINITY;
     }
-    // ---- running maximum ----
-    float mx = sc[0][0];
-#pragma unroll
-    for (int n = 0; n < 2; n++)
-#pragma unroll
-        for (int i = 0; i < 16; i++) mx = fmaxf(mx, sc[n][i]);
-    {
-        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// The largest of v over the lanes of a row.
+template <int M>
+__device__ __forceinline__ float row_max(float v) {
+    if constexpr (M == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
     }
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+template <int M>
+__device__ __forceinline__ float row_sum(float v) {
+    if constexpr (M == 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// The running maximum; O and l rescaled where it grew enough. Returns what the tile's exponents
+// subtract.
+template <int D, int TERMS, int M>
+__device__ __forceinline__ float tile_maximum(RowState<D, TERMS, M>& s, float c) {
+    typedef RowState<D, TERMS, M> S;
+    float mx = s.sc[0][0];
+#pragma unroll
+    for (int n = 0; n < S::NS; n++)
+#pragma unroll
+        for (int i = 0; i < S::E; i++) mx = fmaxf(mx, s.sc[n][i]);
+    mx = row_max<M>(mx);
     if (__any((mx - s.m) * c > T_GROW || s.m == -INFINITY)) {
         const float mn = fmaxf(s.m, mx);
         const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((s.m - mn) * c);
         s.m = mn;
         s.l *= f;
 #pragma unroll
-        for (int d = 0; d < D / 32; d++)
+        for (int d = 0; d < D / M; d++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) s.o[d][i] *= f;
+            for (int i = 0; i < S::E; i++) s.o[d][i] *= f;
     }
     float m0 = s.m == -INFINITY ? 0.0f : s.m;
     if (c > 1.0f) {  // uniform
 #pragma unroll
-        for (int n = 0; n < 2; n++)
+        for (int n = 0; n < S::NS; n++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) sc[n][i] -= m0;
+            for (int i = 0; i < S::E; i++) s.sc[n][i] -= m0;
         m0 = 0.0f;
     }
-    const float mb = m0 * c;
-    // ---- p, its sum, and the products, 16 keys at a time ----
+    return m0 * c;
+}
+
+// The tile's weights p = 2^(s c - mb), their sum, and O += V^T P^T.
+template <int D, int TERMS, int M>
+__device__ __forceinline__ void tile_values(RowState<D, TERMS, M>& s, const uint8_t* vt, float c, float mb, int lane) {
+    typedef TileLay<D> L;
+    typedef RowState<D, TERMS, M> S;
     const tbf16x2 ones = __builtin_bit_cast(tbf16x2, 0x3f803f80u);
-    float sum = 0.0f;
-    const int grp = lane >> 4, r4 = (lane & 15) >> 2;
-    const uint8_t* vrow = vt + (4 * half + r4) * L::ROWB + 8 * (lane & 1);
-    const int vc = 2 * (grp & 1) + ((lane & 3) >> 1), vx = L::vx(4 * half + r4);
+    const int part = lane / M, r4 = (lane & 15) >> 2;
+    const uint8_t* vrow = vt + (4 * part + r4) * L::ROWB + 8 * (lane & 1);
+    const int vc = (M == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1), vx = L::vx(4 * part + r4);
 #pragma unroll
-    for (int n = 0; n < 2; n++) {
-        float p[16];
+    for (int w = 0; w < 64 / S::KD; w++) {
+        // the lane's 8 keys of this product: two runs of four, 256 / M apart
+        float p[8];
 #pragma unroll
-        for (int i = 0; i < 16; i++) p[i] = __builtin_amdgcn_exp2f(fmaf(sc[n][i], c, -mb));
+        for (int j = 0; j < 8; j++) {
+            const int e = 8 * w + j;  // of the lane's E NS scores, in order
+            p[j] = __builtin_amdgcn_exp2f(fmaf(s.sc[e / S::E][e % S::E], c, -mb));
+        }
         if constexpr (TERMS > 1) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) sum += p[i];
+            for (int j = 0; j < 8; j++) s.l += p[j];
+        }
+        tbf16x8 pb[TERMS];
+#pragma unroll
+        for (int t = 0; t < TERMS; t++) {
+            uint32_t b[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                b[j] = t_pack(p[2 * j], p[2 * j + 1]);
+                if (TERMS == 1) s.l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(tbf16x2, b[j]), ones, s.l, false);
+                if (t + 1 < TERMS) {
+                    p[2 * j] -= __uint_as_float(b[j] << 16);  // exact: the remainder of a round to nearest
+                    p[2 * j + 1] -= __uint_as_float(b[j] & 0xffff0000u);
+                }
+            }
+            pb[t] = __builtin_bit_cast(tbf16x8, make_uint4(b[0], b[1], b[2], b[3]));
         }
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            tbf16x8 pb[TERMS];
+        for (int d = 0; d < D / M; d++) {
+            const uint8_t* va = vrow + S::KD * w * L::ROWB + 16 * ((M / 8 * d + vc) ^ vx);
+            const ts16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)va);
+            const ts16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(va + 256 / M * L::ROWB));
+            const uint2 w0 = __builtin_bit_cast(uint2, v0), w1 = __builtin_bit_cast(uint2, v1);
+            const tbf16x8 vv = __builtin_bit_cast(tbf16x8, make_uint4(w0.x, w0.y, w1.x, w1.y));
 #pragma unroll
-            for (int t = 0; t < TERMS; t++) {
-                uint32_t w[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    float &x = p[8 * u + 2 * e], &y = p[8 * u + 2 * e + 1];
-                    w[e] = t_pack(x, y);
-                    if (TERMS == 1) sum = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(tbf16x2, w[e]), ones, sum, false);
-                    if (t + 1 < TERMS) {
-                        x -= __uint_as_float(w[e] << 16);
-                        y -= __uint_as_float(w[e] & 0xffff0000u);
-                    }
-                }
-                pb[t] = __builtin_bit_cast(tbf16x8, make_uint4(w[0], w[1], w[2], w[3]));
-            }
-#pragma unroll
-            for (int d = 0; d < D / 32; d++) {
-                const uint8_t* va = vrow + (32 * n + 16 * u) * L::ROWB + 16 * ((4 * d + vc) ^ vx);
-                const ts16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)va);
-                const ts16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(va + 8 * L::ROWB));
-                const uint2 w0 = __builtin_bit_cast(uint2, v0), w1 = __builtin_bit_cast(uint2, v1);
-                const tbf16x8 vv = __builtin_bit_cast(tbf16x8, make_uint4(w0.x, w0.y, w1.x, w1.y));
-                tbf16x8 vf = vv;
-                if constexpr (MASKED || TERMS > 1) vf = bad_v ? t_finite8(vv) : vv;
-#pragma unroll
-                for (int t = TERMS - 1; t >= 0; t--)
-                    s.o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(MASKED || t > 0 ? vf : vv, pb[t], s.o[d], 0, 0, 0);
-            }
+            for (int t = TERMS - 1; t >= 0; t--) s.o[d] = Mx<M>::mul(vv, pb[t], s.o[d]);
         }
     }
-    s.l += sum;
-    if constexpr (MASKED) {
-        if (bad_v) {  // uniform; rare: infinities and NaN of V reach the rows that see their key
-            const int last = min(s.pos, k1 - 1) - key0;
-            for (int key = 0; key < 64; key++) {
-                if (!__any(key <= last)) break;
+}
+
+// The infinities and NaN of a V tile to the rows that see their key: a hidden key has no part in a
+// row, whatever its value holds, and its weight of zero times an infinity would be NaN.
+template <int D, int TERMS, int M>
+__device__ __forceinline__ void tile_bad_values(RowState<D, TERMS, M>& s, const uint8_t* vt, int last, int lane) {
+    typedef TileLay<D> L;
+    const int part = lane / M;
+    for (int key = 0; key < 64; key++) {
+        if (!__any(key <= last)) break;
 #pragma unroll
-                for (int d = 0; d < D / 32; d++)
+        for (int d = 0; d < D / M; d++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        const int chunk = (4 * d + e) ^ L::vx(key);  // dims 32 d + 8 e + 4 half ..
-                        const uint2 w = *reinterpret_cast<const uint2*>(vt + key * L::ROWB + 16 * chunk + 8 * half);
-                        const uint32_t b0 = w.x & ~t_finite(w.x), b1 = w.y & ~t_finite(w.y);
-                        if (key <= last) {
-                            s.o[d][4 * e] += __uint_as_float(b0 << 16);
-                            s.o[d][4 * e + 1] += __uint_as_float(b0 & 0xffff0000u);
-                            s.o[d][4 * e + 2] += __uint_as_float(b1 << 16);
-                            s.o[d][4 * e + 3] += __uint_as_float(b1 & 0xffff0000u);
-                        }
-                    }
+            for (int e = 0; e < M * M / 256; e++) {
+                const int dim = M * d + (256 / M) * e + 4 * part;
+                const uint2 w = *reinterpret_cast<const uint2*>(vt + key * L::ROWB + 16 * ((dim / 8) ^ L::vx(key)) +
+                                                                2 * (dim & 7));
+                const uint32_t b0 = w.x & ~t_finite(w.x), b1 = w.y & ~t_finite(w.y);
+                if (key <= last) {
+                    s.o[d][4 * e] += __uint_as_float(b0 << 16);
+                    s.o[d][4 * e + 1] += __uint_as_float(b0 & 0xffff0000u);
+                    s.o[d][4 * e + 2] += __uint_as_float(b1 << 16);
+                    s.o[d][4 * e + 3] += __uint_as_float(b1 & 0xffff0000u);
+                }
             }
-        }
     }
 }
 
 // out = O / l of the wave's rows, or their partial (O, m, l) for the merge. A row that sees no key
 // gives zeros.
-template <int D, int TERMS>
-__device__ __forceinline__ void rows_store(RowState<D, TERMS>& s, const TileArgs& a, const AttnItem& it, int h, int wrow,
+template <int D, int TERMS, int M>
+__device__ __forceinline__ void rows_store(RowState<D, TERMS, M>& s, const TileArgs& a, const AttnItem& it, int h, int wrow,
                                            int lane) {
-    const int r = wrow + (lane & 31), half = lane >> 5;
-    {
-        const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(s.l), __float_as_uint(s.l), false, false);
-        s.l = __uint_as_float(x[0]) + __uint_as_float(x[1]);
-    }
+    const int r = wrow + lane % M, part = lane / M;
+    s.l = row_sum<M>(s.l);
     if (!s.live) return;
     if (it.part >= 0) {
         const int64_t pr = (int64_t)h * a.part_rows + it.part + r;
-        if (half == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * pr) = make_float2(s.m, s.l);
+        if (part == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * pr) = make_float2(s.m, s.l);
 #pragma unroll
-        for (int d = 0; d < D / 32; d++)
+        for (int d = 0; d < D / M; d++)
 #pragma unroll
-            for (int e = 0; e < 4; e++)
-                *reinterpret_cast<float4*>(a.part_acc + pr * D + 32 * d + 8 * e + 4 * half) =
+            for (int e = 0; e < M * M / 256; e++)
+                *reinterpret_cast<float4*>(a.part_acc + pr * D + M * d + 256 / M * e + 4 * part) =
                     make_float4(s.o[d][4 * e], s.o[d][4 * e + 1], s.o[d][4 * e + 2], s.o[d][4 * e + 3]);
         return;
     }
     const float inv = s.pos < 0 ? 0.0f : 1.0f / s.l;
     const uint32_t row = (uint32_t)(it.row0 + r), tok = row / (uint32_t)a.G, g = row - tok * a.G;
-    const int64_t at = (int64_t)(it.q0 + (int)tok) * a.out_stride + (int64_t)(h * a.G + (int)g) * D + 4 * half;
+    const int64_t at = (int64_t)(it.q0 + (int)tok) * a.out_stride + (int64_t)(h * a.G + (int)g) * D + 4 * part;
 #pragma unroll
-    for (int d = 0; d < D / 32; d++)
+    for (int d = 0; d < D / M; d++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
+        for (int e = 0; e < M * M / 256; e++) {
             const float x0 = s.o[d][4 * e] * inv, x1 = s.o[d][4 * e + 1] * inv, x2 = s.o[d][4 * e + 2] * inv,
                         x3 = s.o[d][4 * e + 3] * inv;
-            const int64_t i = at + 32 * d + 8 * e;
+            const int64_t i = at + M * d + 256 / M * e;
             if (a.out_dtype == OOM_BF16)
                 *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + i) = make_uint2(t_pack(x0, x1), t_pack(x2, x3));
             else
@@ -434,51 +489,48 @@ __device__ __forceinline__ void rows_store(RowState<D, TERMS>& s, const TileArgs
         }
 }
 
-// Blocks of 4 waves, 32 rows each; block i takes item i / Hkv for KV head i % Hkv (consecutive
-// blocks run on different XCDs, so with 8 KV heads each L2 holds one head's K and V).
+// Blocks of 128 rows, M a wave; block i takes item i / Hkv for KV head i % Hkv (consecutive blocks
+// run on different XCDs, so with 8 KV heads each L2 holds one head's K and V).
 // K and V tiles go through LDS in two stages, one barrier a tile: past it, every wave has done
 // with the stage that the next tile's loads now fill, and those have a whole tile to arrive.
-template <int D, int TERMS, bool PAGED>
-__global__ void __launch_bounds__(256, (D <= 128 && TERMS == 1) ? 2 : 1) attn_tile_kernel(TileArgs a) {
+// Two blocks a CU (d up to 128) or two waves a SIMD take turns on the matrix cores and the
+// vector units.
+template <int D, int TERMS, int M, bool PAGED>
+__global__ void __launch_bounds__(8192 / M, 2) attn_tile_kernel(TileArgs a) {
     typedef TileLay<D> L;
+    constexpr int NW = 128 / M;
     __shared__ __align__(16) uint8_t tiles[4 * L::BYTES];  // stage 0: K, V; stage 1: K, V
     __shared__ uint32_t bad_lds[4];                        // per stage: K, V hold infinities or NaN
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int h = (int)(blockIdx.x % (uint32_t)a.Hkv), item = (int)(blockIdx.x / (uint32_t)a.Hkv);
-    if (item >= a.plan[ATTN_PLAN_ITEMS]) return;
     const AttnItem it = reinterpret_cast<const AttnItem*>(a.plan + ATTN_PLAN_HEAD)[item];
-    const int wrow = 32 * wave;
+    if (item >= a.plan[ATTN_PLAN_ITEMS]) return;
+    const int wrow = M * wave;
     const bool has = wrow < it.rows;  // uniform
     const float c = a.scale * 1.44269504088896340736f;
-    TileSrc<D, PAGED> src;
-    src.init(a, it, h, lane);
+    TileSrc<D, NW, PAGED> src;
+    src.init(a, it, h, lane, wave);
     if (threadIdx.x < 4) bad_lds[threadIdx.x] = 0;
-    const uint32_t mine = (uint32_t)(uintptr_t)(t_lds_t)tiles + 16 * wave * L::ROWB;  // LDS address of the wave's rows
-    const bool any = it.k0 < it.k1;
-    if (any) src.load(it.k0 + 16 * wave, lane, mine, mine + L::BYTES);
-    RowState<D, TERMS> s;
+    const uint32_t mine = (uint32_t)(uintptr_t)(t_lds_t)tiles + wave * (L::BYTES / NW);  // LDS address of the wave's rows
+    constexpr int WR = 64 / NW;                                                       // rows a wave loads
+    if (it.k0 < it.k1) src.load(it.k0 + WR * wave, lane, mine, mine + L::BYTES);
+    RowState<D, TERMS, M> s;
     rows_init(s, a, it, h, wrow, lane);
     __syncthreads();  // bad_lds is cleared
     // the wave's last position; the tiles that every row of the block sees whole come first
-    const int pos_hi = it.off + (int)((uint32_t)(it.row0 + min(wrow + 31, it.rows - 1)) / (uint32_t)a.G);
+    const int pos_hi = it.off + (int)((uint32_t)(it.row0 + min(wrow + M - 1, it.rows - 1)) / (uint32_t)a.G);
     const int block_lo = it.off + (int)((uint32_t)it.row0 / (uint32_t)a.G);
     const int whole = it.k0 + (max(0, min(it.k1, block_lo + 1) - it.k0) & ~63);
     int key0 = it.k0;
     uint32_t stage = 0;
 
-    const auto next = [&]() {
-        if (key0 + 64 < it.k1) {
-            const uint32_t to = mine + (stage ^ (2 * L::BYTES));
-            src.load(key0 + 64 + 16 * wave, lane, to, to + L::BYTES);
-        }
-    };
     // K's (three terms) and V's infinities and NaN in the wave's part of the tile
     const auto look = [&]() {
         uint32_t bk = 0, bv = 0;
 #pragma unroll
-        for (int n = 0; n < D / 32; n++) {
-            const uint8_t* at = tiles + stage + 16 * wave * L::ROWB + n * 1024 + 16 * lane;
+        for (int n = 0; n < L::BYTES / NW / 1024; n++) {
+            const uint8_t* at = tiles + stage + wave * (L::BYTES / NW) + n * 1024 + 16 * lane;
             const uint4 w = *reinterpret_cast<const uint4*>(at + L::BYTES);
             bv |= t_nonfinite(w.x) | t_nonfinite(w.y) | t_nonfinite(w.z) | t_nonfinite(w.w);
             if constexpr (TERMS > 1) {
@@ -491,24 +543,52 @@ __global__ void __launch_bounds__(256, (D <= 128 && TERMS == 1) ? 2 : 1) attn_ti
         if (bv) bad[1] = 1;
         __builtin_amdgcn_s_waitcnt(0xC07F);
     };
-    for (; key0 < whole; key0 += 64, stage ^= 2 * L::BYTES) {
+    const auto step = [&](auto masked_tile) {
+        constexpr bool MASKED = decltype(masked_tile)::value;
+        const uint8_t* const kt = tiles + stage;
+        uint8_t* const vt = tiles + stage + L::BYTES;
         t_wait_loads();
-        if constexpr (TERMS > 1) look();
+        if constexpr (MASKED || TERMS > 1) look();
         t_barrier();
-        next();
-        const bool bad_k = TERMS > 1 && bad_lds[stage ? 2 : 0] != 0, bad_v = TERMS > 1 && bad_lds[stage ? 3 : 1] != 0;
-        if (has) tile_step<D, TERMS, false>(s, tiles + stage, tiles + stage + L::BYTES, key0, it.k1, c, bad_k, bad_v, lane);
-    }
-    for (; key0 < it.k1; key0 += 64, stage ^= 2 * L::BYTES) {
-        t_wait_loads();
-        look();
-        t_barrier();
-        next();
-        const bool bad_k = TERMS > 1 && bad_lds[stage ? 2 : 0] != 0, bad_v = bad_lds[stage ? 3 : 1] != 0;
-        if (has && key0 <= pos_hi)
-            tile_step<D, TERMS, true>(s, tiles + stage, tiles + stage + L::BYTES, key0, it.k1, c, bad_k, bad_v, lane);
-    }
+        if (key0 + 64 < it.k1) {
+            const uint32_t to = mine + (stage ^ (2 * L::BYTES));
+            src.load(key0 + 64 + WR * wave, lane, to, to + L::BYTES);
+        }
+        const bool sees = has && (!MASKED || key0 <= pos_hi);  // uniform
+        const int last = MASKED ? min(s.pos, it.k1 - 1) - key0 : 63;
+        if (sees) {
+            if (TERMS > 1 && bad_lds[stage ? 2 : 0] != 0) tile_scores<D, TERMS, M, MASKED, true>(s, kt, last, lane);
+            else tile_scores<D, TERMS, M, MASKED, false>(s, kt, last, lane);
+        }
+        const float mb = sees ? tile_maximum(s, c) : 0.0f;
+        if ((MASKED || TERMS > 1) && bad_lds[stage ? 3 : 1] != 0) {  // uniform over the block; rare
+            if (sees) tile_bad_values(s, vt, last, lane);
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < L::BYTES / NW / 1024; n++) {
+                uint4* p = reinterpret_cast<uint4*>(vt + wave * (L::BYTES / NW) + n * 1024 + 16 * lane);
+                *p = __builtin_bit_cast(uint4, t_finite8(__builtin_bit_cast(tbf16x8, *p)));
+            }
+            if (threadIdx.x == 0) bad_lds[stage ? 3 : 1] = 0;
+            __syncthreads();
+        }
+        if (sees) tile_values(s, vt, c, mb, lane);
+    };
+    for (; key0 < whole; key0 += 64, stage ^= 2 * L::BYTES) step(std::false_type{});
+    for (; key0 < it.k1; key0 += 64, stage ^= 2 * L::BYTES) step(std::true_type{});
     if (has) rows_store(s, a, it, h, wrow, lane);
+}
+
+// Rows a wave: 32 up to d 128 in one term; 16 for three terms and for d 256, whose Q and O of 32 rows
+// leave no registers for a second wave on the SIMD.
+template <int D, int TERMS>
+constexpr int tile_m() { return D <= 128 && TERMS == 1 ? 32 : 16; }
+
+template <int D, bool PAGED>
+void launch_tiles(const TileArgs& a, dim3 grid, bool exact, hipStream_t st) {
+    constexpr int M1 = tile_m<D, 1>(), M3 = tile_m<D, 3>();
+    if (exact) hipLaunchKernelGGL((attn_tile_kernel<D, 3, M3, PAGED>), grid, dim3(8192 / M3), 0, st, a);
+    else hipLaunchKernelGGL((attn_tile_kernel<D, 1, M1, PAGED>), grid, dim3(8192 / M1), 0, st, a);
 }
 
 }  // namespace oom

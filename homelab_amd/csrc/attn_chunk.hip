@@ -6,54 +6,73 @@
 
 namespace oom {
 
-// Block (x, y): KV head x % Hkv of merge x / Hkv, its rows 16 y .. 16 y + 15, a wave 4 of them in
-// turn. The parts' maxima give their weights e^((m_p - M) scale); out = sum_p w_p O_p / sum_p w_p l_p.
+// The merge of split rows: a wave a (row, KV head), in turn over all of them. The parts' maxima give
+// their weights e^((m_p - M) scale); out = sum_p w_p O_p / sum_p w_p l_p, in part order. The
+// first parts' O are on their way before the weights are known: a row takes two round trips
+// of loads, its entry and then everything.
 template <int D>
 __global__ void __launch_bounds__(256) attn_rows_merge_kernel(TileArgs a, int64_t max_items) {
-    constexpr int CPL = D / 64;  // columns a lane
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int h = (int)(blockIdx.x % (uint32_t)a.Hkv), m = (int)(blockIdx.x / (uint32_t)a.Hkv);
-    if (m >= a.plan[ATTN_PLAN_MERGES]) return;
-    const int32_t* e = a.plan + ATTN_PLAN_HEAD + (max_items + m) * ATTN_ITEM_WORDS;
+    constexpr int CPL = D / 64, EARLY = 8;  // columns a lane, parts loaded at once
+    typedef float cols_t __attribute__((ext_vector_type(CPL)));
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
+    const int64_t all = (int64_t)a.plan[ATTN_PLAN_MERGES] * a.Hkv;
+    const int4* rows = reinterpret_cast<const int4*>(a.plan + ATTN_PLAN_HEAD + max_items * ATTN_ITEM_WORDS);
     const float c = a.scale * 1.44269504088896340736f;
-    const int q0 = e[0], row0 = e[1], rows = e[2], off = e[3], part = e[4], n = e[5];
-    for (int r = 16 * blockIdx.y + wave; r < min(rows, 16 * (int)blockIdx.y + 16); r += 4) {
-        const int64_t pr = (int64_t)h * a.part_rows + part + r;  // part i's row: + i rows
-        float M = -INFINITY, L = 0.0f, A[CPL] = {};
-        for (int i = lane; i < n; i += 64) M = fmaxf(M, a.part_ml[2 * (pr + (int64_t)i * rows)]);
+    for (int64_t i = wave; i < all; i += gridDim.x * 4) {
+        const int h = (int)(i % a.Hkv);
+        const int4 e = rows[i / a.Hkv];
+        const int n = e.w & 0xffff, stride = e.w >> 16;
+        const int64_t pr = (int64_t)h * a.part_rows + e.z;
+        const float* acc = a.part_acc + pr * D + CPL * lane;
+        cols_t v[EARLY], A = {};
+#pragma unroll
+        for (int j = 0; j < EARLY; j++)
+            if (j < n) v[j] = *reinterpret_cast<const cols_t*>(acc + (int64_t)j * stride * D);  // uniform
+        float M = -INFINITY, L = 0.0f;
+        for (int p0 = 0; p0 < n; p0 += 64)
+            if (p0 + lane < n) M = fmaxf(M, a.part_ml[2 * (pr + (int64_t)(p0 + lane) * stride)]);
         M = wave_max(M);
-        for (int i0 = 0; i0 < n; i0 += 64) {
+        for (int p0 = 0; p0 < n; p0 += 64) {
             float w = 0.0f, l = 0.0f;
-            if (i0 + lane < n) {
-                const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (pr + (int64_t)(i0 + lane) * rows));
+            if (p0 + lane < n) {
+                const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + 2 * (pr + (int64_t)(p0 + lane) * stride));
                 w = ml.x == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f((ml.x - M) * c);
                 l = ml.y * w;
             }
             L += wave_sum(l);
-            for (int i = 0; i < min(64, n - i0); i++) {
-                const float wi = __shfl(w, i);
-                const float* p = a.part_acc + (pr + (int64_t)(i0 + i) * rows) * D + CPL * lane;
+            const int m = min(64, n - p0);
+            for (int j0 = 0; j0 < m; j0 += EARLY) {
+                if (p0 + j0 > 0)
 #pragma unroll
-                for (int j = 0; j < CPL; j++) A[j] = fmaf(p[j], wi, A[j]);
+                    for (int j = 0; j < EARLY; j++)
+                        if (p0 + j0 + j < n)
+                            v[j] = *reinterpret_cast<const cols_t*>(acc + (int64_t)(p0 + j0 + j) * stride * D);
+#pragma unroll
+                for (int j = 0; j < EARLY; j++) {
+                    if (j0 + j >= m) break;
+                    const float wj = __shfl(w, j0 + j);
+#pragma unroll
+                    for (int x = 0; x < CPL; x++) A[x] = fmaf(v[j][x], wj, A[x]);
+                }
             }
         }
-        const uint32_t row = (uint32_t)(row0 + r), tok = row / (uint32_t)a.G, g = row - tok * a.G;
-        const float inv = off + (int)tok < 0 ? 0.0f : 1.0f / L;
-        const int64_t at = (int64_t)(q0 + (int)tok) * a.out_stride + (int64_t)(h * a.G + (int)g) * D + CPL * lane;
+        const float inv = e.y >> 30 ? 0.0f : 1.0f / L;
+        const int64_t at = (int64_t)e.x * a.out_stride + (int64_t)(h * a.G + (e.y & 0xffff)) * D + CPL * lane;
 #pragma unroll
-        for (int j = 0; j < CPL; j++) {
-            if (a.out_dtype == OOM_BF16) store_out<OOM_BF16>(a.out, at + j, A[j] * inv);
-            else store_out<OOM_F32>(a.out, at + j, A[j] * inv);
+        for (int x = 0; x < CPL; x++) {
+            if (a.out_dtype == OOM_BF16) store_out<OOM_BF16>(a.out, at + x, A[x] * inv);
+            else store_out<OOM_F32>(a.out, at + x, A[x] * inv);
         }
     }
 }
 
 template <int D>
-static int launch_chunk(const TileArgs& a, const AttnPlanDims& p, int64_t rows, bool exact, hipStream_t st) {
+static int launch_chunk(const TileArgs& a, const AttnPlanDims& p, bool exact, hipStream_t st) {
     const dim3 grid((uint32_t)(p.items * a.Hkv));
     launch_tiles<D, true>(a, grid, exact, st);
     if (int rc = launched("oom_attn_chunk_paged")) return rc;
-    const dim3 mgrid((uint32_t)(p.merges * a.Hkv), (uint32_t)cdiv(std::min<int64_t>(rows, ATTN_ROWS), 16));
+    const dim3 mgrid((uint32_t)std::min<int64_t>(2048, cdiv(p.merge_rows * a.Hkv, 4)));
     hipLaunchKernelGGL((attn_rows_merge_kernel<D>), mgrid, dim3(256), 0, st, a, p.items);
     return launched("oom_attn_chunk_paged");
 }
@@ -117,9 +136,8 @@ extern "C" int oom_attn_chunk_paged(const void* q, int q_dtype, int64_t q_stride
     a.part_acc = reinterpret_cast<float*>(ws);
     a.part_ml = a.part_acc + p.part_rows * kv_heads * d;
     const bool exact = q_dtype == OOM_F32 || out_dtype == OOM_F32;
-    const int64_t rows = (int64_t)T * a.G;
     hipStream_t st = as_stream(stream);
-    if (d == 64) return launch_chunk<64>(a, p, rows, exact, st);
-    if (d == 128) return launch_chunk<128>(a, p, rows, exact, st);
-    return launch_chunk<256>(a, p, rows, exact, st);
+    if (d == 64) return launch_chunk<64>(a, p, exact, st);
+    if (d == 128) return launch_chunk<128>(a, p, exact, st);
+    return launch_chunk<256>(a, p, exact, st);
 }

@@ -12,7 +12,7 @@ struct PlanArgs {
     const int32_t* kv_lens;  // null: prompts, whose keys are their own tokens
     const int32_t* table;
     int max_pages, n_pages, page_size, B, T, G, Hkv;
-    int64_t max_items, max_merges, max_part_rows;
+    int64_t max_items, max_merge_rows, max_part_rows;
     int32_t* positions;
     int64_t* slots;
     int32_t* plan;
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) attn_plan_kernel(PlanArgs a) {
     if (tid < PLAN_BUCKETS) hist[tid] = first;
     __syncthreads();
     int32_t* const list = a.plan + ATTN_PLAN_HEAD;
-    int32_t* const merges = list + a.max_items * ATTN_ITEM_WORDS;
+    int4* const merges = reinterpret_cast<int4*>(list + a.max_items * ATTN_ITEM_WORDS);
     for (int t = tid; t < tiles; t += PLAN_THREADS) {
         const PlanTile p = plan_tile(a, pre, t);
         if (p.rows == 0) continue;
@@ -175,11 +175,14 @@ __global__ void __launch_bounds__(PLAN_THREADS) attn_plan_kernel(PlanArgs a) {
         int part = -1;
         if (ns > 1) {
             part = atomicAdd(&n_parts, ns * p.rows);
-            const int m = atomicAdd(&n_merges, 1);
-            if (part + (int64_t)ns * p.rows > a.max_part_rows || m >= a.max_merges) continue;
-            int32_t* e = merges + (int64_t)m * ATTN_ITEM_WORDS;
-            *reinterpret_cast<int4*>(e) = make_int4(p.q0, p.row0, p.rows, p.off);
-            *reinterpret_cast<int4*>(e + 4) = make_int4(part, ns, 0, 0);
+            const int m = atomicAdd(&n_merges, p.rows);
+            if (part + (int64_t)ns * p.rows > a.max_part_rows || m + (int64_t)p.rows > a.max_merge_rows) continue;
+            // a row to merge: its token, its head of the group (bit 30: it sees no key), its first
+            // partial, and how many there are, p.rows apart
+            for (int r = 0; r < p.rows; r++) {
+                const int tok = (p.row0 + r) / a.G, g = p.row0 + r - tok * a.G;
+                merges[m + r] = make_int4(p.q0 + tok, g | (p.off + tok < 0 ? 1 << 30 : 0), part + r, ns | p.rows << 16);
+            }
         }
         for (int i = 0; i < ns; i++) {
             const int k0 = i * ks * ATTN_KEYS, k1 = min(p.keys, k0 + ks * ATTN_KEYS);
@@ -193,7 +196,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) attn_plan_kernel(PlanArgs a) {
     __syncthreads();
     if (tid == 0) {
         a.plan[ATTN_PLAN_ITEMS] = (int)min((int64_t)items, a.max_items);
-        a.plan[ATTN_PLAN_MERGES] = (int)min((int64_t)n_merges, a.max_merges);
+        a.plan[ATTN_PLAN_MERGES] = (int)min((int64_t)n_merges, a.max_merge_rows);
     }
 }
 
@@ -235,7 +238,7 @@ extern "C" int oom_attn_plan(const int32_t* cu_q, const int32_t* kv_lens, const 
     a.G = heads / kv_heads;
     a.Hkv = kv_heads;
     a.max_items = p.items;
-    a.max_merges = p.merges;
+    a.max_merge_rows = p.merge_rows;
     a.max_part_rows = p.part_rows;
     a.positions = positions;
     a.slots = slots;

@@ -302,26 +302,26 @@ constexpr int ATTN_SPLIT_BLOCKS = 512;  // blocks that a batch's keys are split 
 constexpr int ATTN_MAXB = 4096;       // sequences of a plan
 constexpr int ATTN_MAX_KEYS = 1 << 27;  // keys of a sequence
 
-// A plan in i32 words: ATTN_PLAN_HEAD words of counts, then the items, then the merges.
+// A plan in i32 words: ATTN_PLAN_HEAD words of counts, then the items, then the rows to merge.
 constexpr int ATTN_PLAN_HEAD = 16;
-constexpr int ATTN_ITEM_WORDS = 8;
-constexpr int ATTN_PLAN_ITEMS = 0, ATTN_PLAN_MERGES = 1;  // head words: items, merges
+constexpr int ATTN_ITEM_WORDS = 8, ATTN_MERGE_WORDS = 4;
+constexpr int ATTN_PLAN_ITEMS = 0, ATTN_PLAN_MERGES = 1;  // head words: items, rows to merge
 
 // The plan's bounds, from sizes that the host knows. Tiles of sequence b: ceil(n_b G / 128), so at
 // most T G / 128 + B in all. With W key tiles over them and splits of ks = ceil(W Hkv / 512),
 // the items number at most tiles + W / ks and the tiles that are split at all (more than ks
 // key tiles) at most W / ks <= ceil(512 / Hkv); their parts at most twice that.
 struct AttnPlanDims {
-    int64_t tiles, items, merges, part_rows, words;
+    int64_t tiles, items, merge_rows, part_rows, words;
 };
 inline AttnPlanDims attn_plan_dims(int64_t T, int64_t B, int heads, int kv_heads) {
     AttnPlanDims p;
     const int64_t rows = T * (heads / kv_heads), split = cdiv(ATTN_SPLIT_BLOCKS, kv_heads);
     p.tiles = rows / ATTN_ROWS + B;
     p.items = p.tiles + split;
-    p.merges = split;
+    p.merge_rows = std::min<int64_t>(split * ATTN_ROWS, rows);
     p.part_rows = 2 * split * std::min<int64_t>(ATTN_ROWS, std::max<int64_t>(rows, 1));
-    p.words = ATTN_PLAN_HEAD + (p.items + p.merges) * ATTN_ITEM_WORDS;
+    p.words = ATTN_PLAN_HEAD + p.items * ATTN_ITEM_WORDS + p.merge_rows * ATTN_MERGE_WORDS;
     return p;
 }
 

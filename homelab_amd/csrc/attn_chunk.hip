@@ -2,33 +2,36 @@
 // over pages, then the merge of the row tiles whose keys were split.
 #include <cmath>
 
-#include "attn_tile.hpp"
+#include "attn_few.hpp"
 
 namespace oom {
 
 // The merge of split rows: a wave a (row, KV head), in turn over all of them. The parts' maxima give
-// their weights e^((m_p - M) scale); out = sum_p w_p O_p / sum_p w_p l_p, in part order. The
-// first parts' O are on their way before the weights are known: a row takes two round trips
-// of loads, its entry and then everything.
+// their weights e^((m_p - M) scale); out = sum_p w_p O_p / sum_p w_p l_p. A load takes the row of
+// 256 / d parts, 16 bytes a lane; the first 16 loads' parts are on their way before the weights
+// are known, so a row takes two round trips, its entry and then everything.
 template <int D>
-__global__ void __launch_bounds__(256) attn_rows_merge_kernel(TileArgs a, int64_t max_items) {
-    constexpr int CPL = D / 64, EARLY = 8;  // columns a lane, parts loaded at once
-    typedef float cols_t __attribute__((ext_vector_type(CPL)));
-    const int lane = threadIdx.x & 63;
+__global__ void __launch_bounds__(256) attn_rows_merge_kernel(TileArgs a, const int4* rows) {
+    constexpr int LPP = D / 4, PP = 64 / LPP, EARLY = 16;  // lanes a part, parts a load, loads at once
+    const int lane = threadIdx.x & 63, sub = lane / LPP, col = lane % LPP * 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
     const int64_t all = (int64_t)a.plan[ATTN_PLAN_MERGES] * a.Hkv;
-    const int4* rows = reinterpret_cast<const int4*>(a.plan + ATTN_PLAN_HEAD + max_items * ATTN_ITEM_WORDS);
     const float c = a.scale * 1.44269504088896340736f;
     for (int64_t i = wave; i < all; i += gridDim.x * 4) {
         const int h = (int)(i % a.Hkv);
         const int4 e = rows[i / a.Hkv];
         const int n = e.w & 0xffff, stride = e.w >> 16;
         const int64_t pr = (int64_t)h * a.part_rows + e.z;
-        const float* acc = a.part_acc + pr * D + CPL * lane;
-        cols_t v[EARLY], A = {};
+        const float* acc = a.part_acc + pr * D + col;
+        float4 v[EARLY];
+        float A[4] = {};
+        const auto load = [&](int p0) {
 #pragma unroll
-        for (int j = 0; j < EARLY; j++)
-            if (j < n) v[j] = *reinterpret_cast<const cols_t*>(acc + (int64_t)j * stride * D);  // uniform
+            for (int j = 0; j < EARLY; j++)
+                if (p0 + PP * j < n)  // uniform
+                    v[j] = *reinterpret_cast<const float4*>(acc + (int64_t)min(p0 + PP * j + sub, n - 1) * stride * D);
+        };
+        load(0);
         float M = -INFINITY, L = 0.0f;
         for (int p0 = 0; p0 < n; p0 += 64)
             if (p0 + lane < n) M = fmaxf(M, a.part_ml[2 * (pr + (int64_t)(p0 + lane) * stride)]);
@@ -41,39 +44,53 @@ __global__ void __launch_bounds__(256) attn_rows_merge_kernel(TileArgs a, int64_
                 l = ml.y * w;
             }
             L += wave_sum(l);
-            const int m = min(64, n - p0);
-            for (int j0 = 0; j0 < m; j0 += EARLY) {
-                if (p0 + j0 > 0)
-#pragma unroll
-                    for (int j = 0; j < EARLY; j++)
-                        if (p0 + j0 + j < n)
-                            v[j] = *reinterpret_cast<const cols_t*>(acc + (int64_t)(p0 + j0 + j) * stride * D);
+            for (int q0 = 0; q0 < min(64, n - p0); q0 += PP * EARLY) {
+                if (p0 + q0 > 0) load(p0 + q0);
 #pragma unroll
                 for (int j = 0; j < EARLY; j++) {
-                    if (j0 + j >= m) break;
-                    const float wj = __shfl(w, j0 + j);
-#pragma unroll
-                    for (int x = 0; x < CPL; x++) A[x] = fmaf(v[j][x], wj, A[x]);
+                    const int p = q0 + PP * j + sub;
+                    const float wj = __shfl(w, p & 63);
+                    if (p < 64 && p0 + p < n) {
+                        A[0] = fmaf(v[j].x, wj, A[0]);
+                        A[1] = fmaf(v[j].y, wj, A[1]);
+                        A[2] = fmaf(v[j].z, wj, A[2]);
+                        A[3] = fmaf(v[j].w, wj, A[3]);
+                    }
                 }
             }
         }
-        const float inv = e.y >> 30 ? 0.0f : 1.0f / L;
-        const int64_t at = (int64_t)e.x * a.out_stride + (int64_t)(h * a.G + (e.y & 0xffff)) * D + CPL * lane;
 #pragma unroll
-        for (int x = 0; x < CPL; x++) {
-            if (a.out_dtype == OOM_BF16) store_out<OOM_BF16>(a.out, at + x, A[x] * inv);
-            else store_out<OOM_F32>(a.out, at + x, A[x] * inv);
-        }
+        for (int o = 32; o >= LPP; o >>= 1)
+#pragma unroll
+            for (int x = 0; x < 4; x++) A[x] += lane_xor_n(A[x], o, lane);
+        if (sub > 0) continue;
+        const float inv = e.y >> 30 ? 0.0f : 1.0f / L;
+        const int64_t at = (int64_t)e.x * a.out_stride + (int64_t)(h * a.G + (e.y & 0xffff)) * D + col;
+        if (a.out_dtype == OOM_BF16)
+            *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + at) =
+                make_uint2(t_pack(A[0] * inv, A[1] * inv), t_pack(A[2] * inv, A[3] * inv));
+        else
+            *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + at) =
+                make_float4(A[0] * inv, A[1] * inv, A[2] * inv, A[3] * inv);
     }
 }
 
+// The kernels that a batch may need: sequences of more than attn_few_rows() rows there are only where max_q new
+// tokens have them, few-row ones only beside others, or where max_q leaves no others.
 template <int D>
-static int launch_chunk(const TileArgs& a, const AttnPlanDims& p, bool exact, hipStream_t st) {
-    const dim3 grid((uint32_t)(p.items * a.Hkv));
-    launch_tiles<D, true>(a, grid, exact, st);
-    if (int rc = launched("oom_attn_chunk_paged")) return rc;
-    const dim3 mgrid((uint32_t)std::min<int64_t>(2048, cdiv(p.merge_rows * a.Hkv, 4)));
-    hipLaunchKernelGGL((attn_rows_merge_kernel<D>), mgrid, dim3(256), 0, st, a, p.items);
+static int launch_chunk(const TileArgs& a, const AttnPlanDims& p, int B, int max_q, bool exact, hipStream_t st) {
+    const int64_t most = (int64_t)max_q * a.G;
+    if (most > attn_few_rows(D)) {
+        launch_tiles<D, true>(a, dim3((uint32_t)(p.items * a.Hkv)), exact, st);
+        if (int rc = launched("oom_attn_chunk_paged")) return rc;
+    }
+    if (most <= attn_few_rows(D) || B > 1) {
+        launch_few<D>(a, p, exact, st);
+        if (int rc = launched("oom_attn_chunk_paged")) return rc;
+    }
+    const int4* rows = reinterpret_cast<const int4*>(a.plan + ATTN_PLAN_HEAD + (p.items + p.few_items) * ATTN_ITEM_WORDS);
+    const dim3 grid((uint32_t)std::min<int64_t>(2048, cdiv(p.merge_rows * a.Hkv, 4)));
+    hipLaunchKernelGGL((attn_rows_merge_kernel<D>), grid, dim3(256), 0, st, a, rows);
     return launched("oom_attn_chunk_paged");
 }
 
@@ -81,7 +98,7 @@ static int launch_chunk(const TileArgs& a, const AttnPlanDims& p, bool exact, hi
 
 extern "C" size_t oom_attn_chunk_paged_workspace_size(int T, int B, int heads, int kv_heads, int d) {
     if (T < 0 || B < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || d < 1) return 0;
-    return (size_t)oom::attn_plan_dims(T, B, heads, kv_heads).part_rows * kv_heads * (d + 2) * sizeof(float) + 256;
+    return (size_t)oom::attn_plan_dims(T, B, heads, kv_heads, d).part_rows * kv_heads * (d + 2) * sizeof(float) + 256;
 }
 
 extern "C" int oom_attn_chunk_paged(const void* q, int q_dtype, int64_t q_stride, const uint16_t* k_pages,
@@ -109,7 +126,7 @@ extern "C" int oom_attn_chunk_paged(const void* q, int q_dtype, int64_t q_stride
     OOM_REQUIRE(q && k_pages && v_pages && page_table && plan && out, "oom_attn_chunk_paged: null buffer");
     OOM_REQUIRE(aligned(q, 16) && aligned(k_pages, 16) && aligned(v_pages, 16) && aligned(out, 16) && aligned(plan, 16),
                 "oom_attn_chunk_paged: q, k_pages, v_pages, out and plan must be 16-byte aligned");
-    const AttnPlanDims p = attn_plan_dims(T, B, heads, kv_heads);
+    const AttnPlanDims p = attn_plan_dims(T, B, heads, kv_heads, d);
     OOM_REQUIRE(p.items * kv_heads < (1ll << 31), "oom_attn_chunk_paged: too many tiles of rows");
     if (!ws || ws_bytes < oom_attn_chunk_paged_workspace_size(T, B, heads, kv_heads, d))
         return fail(OOM_ERR_WORKSPACE,
@@ -137,7 +154,7 @@ extern "C" int oom_attn_chunk_paged(const void* q, int q_dtype, int64_t q_stride
     a.part_ml = a.part_acc + p.part_rows * kv_heads * d;
     const bool exact = q_dtype == OOM_F32 || out_dtype == OOM_F32;
     hipStream_t st = as_stream(stream);
-    if (d == 64) return launch_chunk<64>(a, p, exact, st);
-    if (d == 128) return launch_chunk<128>(a, p, exact, st);
-    return launch_chunk<256>(a, p, exact, st);
+    if (d == 64) return launch_chunk<64>(a, p, B, max_q, exact, st);
+    if (d == 128) return launch_chunk<128>(a, p, B, max_q, exact, st);
+    return launch_chunk<256>(a, p, B, max_q, exact, st);
 }

@@ -1,7 +1,8 @@
 // The attention plan of one step's batch, made once on the device and used by every layer:
 // the tiles of 128 packed query rows of each sequence with the keys that they see, split over
 // the keys where there are too few of them to fill the chip, longest first (blocks start in
-// order, so the short ones fill the gaps at the end). Also the new tokens' positions and
+// order, so the short ones fill the gaps at the end); sequences of at most 32 rows over a paged cache
+// in a list of their own (attn_few.hpp). Also the new tokens' positions and
 // cache slots, which the rotary and append kernels take.
 #include "common.hpp"
 
@@ -11,8 +12,8 @@ struct PlanArgs {
     const int32_t* cu_q;
     const int32_t* kv_lens;  // null: prompts, whose keys are their own tokens
     const int32_t* table;
-    int max_pages, n_pages, page_size, B, T, G, Hkv;
-    int64_t max_items, max_merge_rows, max_part_rows;
+    int max_pages, n_pages, page_size, B, T, G, Hkv, few_rows;
+    int64_t max_items, max_few, max_merge_rows, max_part_rows;
     int32_t* positions;
     int64_t* slots;
     int32_t* plan;
@@ -34,31 +35,6 @@ __device__ __forceinline__ PlanSeq plan_seq(const PlanArgs& a, int b) {
 constexpr int PLAN_THREADS = 1024;
 constexpr int PLAN_BUCKETS = 256;
 
-// Tile t's sequence and its row range and keys; rows 0 where cu_q does not rise and the tile falls
-// outside its sequence.
-struct PlanTile {
-    int b, q0, row0, rows, off, keys, nkt;
-};
-__device__ __forceinline__ PlanTile plan_tile(const PlanArgs& a, const int* pre, int t) {
-    int lo = 0, hi = a.B;  // pre[lo] <= t < pre[hi]
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (pre[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    const PlanSeq s = plan_seq(a, lo);
-    PlanTile p;
-    p.b = lo;
-    p.q0 = s.q0;
-    const int64_t row0 = (int64_t)(t - pre[lo]) * ATTN_ROWS, rows = (int64_t)s.n * a.G - row0;
-    p.row0 = (int)row0;
-    p.rows = row0 < 0 || rows < 0 ? 0 : (int)min((int64_t)ATTN_ROWS, rows);
-    p.off = s.kv - s.n;
-    p.keys = max(0, p.off + (p.row0 + p.rows - 1) / a.G + 1);
-    p.nkt = (p.keys + ATTN_KEYS - 1) / ATTN_KEYS;
-    return p;
-}
-
 // Exclusive prefix sums of v over the block's threads; `total` the whole.
 __device__ int block_scan(int v, int* tmp, int& total) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -79,9 +55,16 @@ __device__ int block_scan(int v, int* tmp, int& total) {
     return before + x - v;
 }
 
+// A tile of rows with its keys; rows 0 where cu_q does not rise and the tile falls outside its
+// sequence. few: the sequence's only tile, its keys in units of ATTN_FEW_KEYS.
+struct PlanTile {
+    int b, q0, row0, rows, off, keys, unit, n;
+    bool few;
+};
+
 // Block 0 writes the items; the blocks after it the positions and slots of 1024 tokens each.
 __global__ void __launch_bounds__(PLAN_THREADS) attn_plan_kernel(PlanArgs a) {
-    const int tid = threadIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63;
     if (blockIdx.x > 0) {
         const int t = (int)(blockIdx.x - 1) * PLAN_THREADS + tid;
         if (t >= a.T) return;
@@ -106,25 +89,31 @@ __global__ void __launch_bounds__(PLAN_THREADS) attn_plan_kernel(PlanArgs a) {
         }
         return;
     }
-    __shared__ int pre[ATTN_MAXB + 1], tmp[PLAN_THREADS / 64], hist[PLAN_BUCKETS];
-    __shared__ unsigned long long work;
-    __shared__ int longest, n_parts, n_merges;
+    __shared__ int pre[ATTN_MAXB + 1], seq_q0[ATTN_MAXB], seq_n[ATTN_MAXB], seq_kv[ATTN_MAXB];
+    __shared__ int tmp[PLAN_THREADS / 64], hist[2][PLAN_BUCKETS];
+    __shared__ unsigned long long work[2];
+    __shared__ int longest[2], n_parts, n_merges;
     constexpr int PER = ATTN_MAXB / PLAN_THREADS;
+    for (int b = tid; b < a.B; b += PLAN_THREADS) {
+        const PlanSeq s = plan_seq(a, b);
+        seq_q0[b] = s.q0;
+        seq_n[b] = s.n;
+        seq_kv[b] = s.kv;
+    }
+    if (tid < 2) {
+        work[tid] = 0;
+        longest[tid] = 1;
+    }
+    if (tid == 0) n_parts = n_merges = pre[0] = 0;
+    if (tid < 2 * PLAN_BUCKETS) (&hist[0][0])[tid] = 0;
+    __syncthreads();
     int mine[PER], sum = 0, tiles;
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         const int b = tid * PER + i;
-        mine[i] = 0;
-        if (b < a.B) mine[i] = (int)(((int64_t)plan_seq(a, b).n * a.G + ATTN_ROWS - 1) / ATTN_ROWS);
+        mine[i] = b < a.B ? (int)(((int64_t)seq_n[b] * a.G + ATTN_ROWS - 1) / ATTN_ROWS) : 0;
         sum += mine[i];
     }
-    if (tid == 0) {
-        work = 0;
-        longest = 1;
-        n_parts = n_merges = 0;
-        pre[0] = 0;
-    }
-    if (tid < PLAN_BUCKETS) hist[tid] = 0;
     int at = block_scan(sum, tmp, tiles);
 #pragma unroll
     for (int i = 0; i < PER; i++) {
@@ -135,67 +124,113 @@ __global__ void __launch_bounds__(PLAN_THREADS) attn_plan_kernel(PlanArgs a) {
     // a batch whose cu_q does not rise can claim more rows than there are: what the plan has no
     // room for is left out
     tiles = (int)min((int64_t)tiles, a.max_items);
-    unsigned long long w = 0;
-    int most = 1;
-    for (int t = tid; t < tiles; t += PLAN_THREADS) {
-        const PlanTile p = plan_tile(a, pre, t);
-        if (p.rows == 0) continue;
-        w += p.nkt;
-        most = max(most, p.nkt);
-    }
-    atomicAdd(&work, w);
-    atomicMax(&longest, most);
-    __syncthreads();
-    // prompts are not split: their rows alone fill the chip, or their keys are few
-    int ks = longest;
-    if (a.kv_lens) {
-        const unsigned long long k = (work * a.Hkv + ATTN_SPLIT_BLOCKS - 1) / ATTN_SPLIT_BLOCKS;
-        ks = (int)min((unsigned long long)longest, max(k, 4ull));
-    }
-    const auto bucket = [&](int n) { return PLAN_BUCKETS - 1 - (int)((int64_t)n * (PLAN_BUCKETS - 1) / ks); };
-    for (int t = tid; t < tiles; t += PLAN_THREADS) {
-        const PlanTile p = plan_tile(a, pre, t);
-        if (p.rows == 0) continue;
-        const int n = p.nkt, ns = max(1, (n + ks - 1) / ks);
-        if (ns > 1) atomicAdd(&hist[0], ns - 1);
-        atomicAdd(&hist[bucket(n - (ns - 1) * ks)], 1);
-    }
-    __syncthreads();
-    int items;
-    const int h = tid < PLAN_BUCKETS ? hist[tid] : 0;
-    const int first = block_scan(h, tmp, items);
-    if (tid < PLAN_BUCKETS) hist[tid] = first;
-    __syncthreads();
-    int32_t* const list = a.plan + ATTN_PLAN_HEAD;
-    int4* const merges = reinterpret_cast<int4*>(list + a.max_items * ATTN_ITEM_WORDS);
-    for (int t = tid; t < tiles; t += PLAN_THREADS) {
-        const PlanTile p = plan_tile(a, pre, t);
-        if (p.rows == 0) continue;
-        const int ns = max(1, (p.nkt + ks - 1) / ks);
-        int part = -1;
-        if (ns > 1) {
-            part = atomicAdd(&n_parts, ns * p.rows);
-            const int m = atomicAdd(&n_merges, p.rows);
-            if (part + (int64_t)ns * p.rows > a.max_part_rows || m + (int64_t)p.rows > a.max_merge_rows) continue;
-            // a row to merge: its token, its head of the group (bit 30: it sees no key), its first
-            // partial, and how many there are, p.rows apart
-            for (int r = 0; r < p.rows; r++) {
-                const int tok = (p.row0 + r) / a.G, g = p.row0 + r - tok * a.G;
-                merges[m + r] = make_int4(p.q0 + tok, g | (p.off + tok < 0 ? 1 << 30 : 0), part + r, ns | p.rows << 16);
-            }
+    const auto tile = [&](int t) {
+        int lo = 0, hi = a.B;  // pre[lo] <= t < pre[hi]
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (pre[mid] <= t) lo = mid;
+            else hi = mid;
         }
-        for (int i = 0; i < ns; i++) {
-            const int k0 = i * ks * ATTN_KEYS, k1 = min(p.keys, k0 + ks * ATTN_KEYS);
-            const int at = atomicAdd(&hist[i + 1 < ns ? 0 : bucket(p.nkt - (ns - 1) * ks)], 1);
-            if (at >= a.max_items) continue;
-            int32_t* e = list + (int64_t)at * ATTN_ITEM_WORDS;
-            *reinterpret_cast<int4*>(e) = make_int4(p.q0, p.row0, p.rows, p.off);
-            *reinterpret_cast<int4*>(e + 4) = make_int4(k0, k1, ns > 1 ? part + i * p.rows : -1, p.b);
+        PlanTile p;
+        p.b = lo;
+        p.q0 = seq_q0[lo];
+        const int64_t all = (int64_t)seq_n[lo] * a.G, row0 = (int64_t)(t - pre[lo]) * ATTN_ROWS, rows = all - row0;
+        p.row0 = (int)row0;
+        p.rows = row0 < 0 || rows < 0 ? 0 : (int)min((int64_t)ATTN_ROWS, rows);
+        p.off = seq_kv[lo] - seq_n[lo];
+        p.keys = max(0, p.off + (p.row0 + p.rows - 1) / a.G + 1);
+        p.few = a.kv_lens && all <= a.few_rows;
+        p.unit = p.few ? ATTN_FEW_KEYS : ATTN_KEYS;
+        p.n = (p.keys + p.unit - 1) / p.unit;
+        return p;
+    };
+    for (int t = tid; t < tiles; t += PLAN_THREADS) {
+        const PlanTile p = tile(t);
+        if (p.rows == 0) continue;
+        atomicAdd(&work[p.few], (unsigned long long)p.n);
+        atomicMax(&longest[p.few], p.n);
+    }
+    __syncthreads();
+    // units a split. Prompts are not split: their rows alone fill the chip, or their keys are few
+    int ks[2] = {longest[0], longest[1]};
+    if (a.kv_lens) {
+        const unsigned long long k0 = (work[0] * a.Hkv + ATTN_SPLIT_BLOCKS - 1) / ATTN_SPLIT_BLOCKS;
+        const unsigned long long k1 = (work[1] * a.Hkv + ATTN_FEW_BLOCKS - 1) / ATTN_FEW_BLOCKS;
+        ks[0] = (int)min((unsigned long long)longest[0], max(k0, 4ull));
+        ks[1] = (int)min((unsigned long long)longest[1], max(k1, 1ull));
+    }
+    const auto splits = [&](const PlanTile& p) { return max(1, (p.n + ks[p.few] - 1) / ks[p.few]); };
+    const auto bucket = [&](const PlanTile& p, int n) {
+        return PLAN_BUCKETS - 1 - (int)((int64_t)n * (PLAN_BUCKETS - 1) / ks[p.few]);
+    };
+    for (int t = tid; t < tiles; t += PLAN_THREADS) {
+        const PlanTile p = tile(t);
+        if (p.rows == 0) continue;
+        const int ns = splits(p);
+        if (ns > 1) atomicAdd(&hist[p.few][0], ns - 1);
+        atomicAdd(&hist[p.few][bucket(p, p.n - (ns - 1) * ks[p.few])], 1);
+    }
+    __syncthreads();
+    int items[2];
+    for (int f = 0; f < 2; f++) {
+        const int h = tid < PLAN_BUCKETS ? hist[f][tid] : 0;
+        const int first = block_scan(h, tmp, items[f]);
+        if (tid < PLAN_BUCKETS) hist[f][tid] = first;
+        __syncthreads();
+    }
+    int32_t* const list = a.plan + ATTN_PLAN_HEAD;
+    int32_t* const few_list = list + a.max_items * ATTN_ITEM_WORDS;
+    int4* const merges = reinterpret_cast<int4*>(few_list + a.max_few * ATTN_ITEM_WORDS);
+    // tile p's split i
+    const auto put = [&](const PlanTile& p, int i, int ns, int part) {
+        const int len = ks[p.few] * p.unit;
+        const int at = atomicAdd(&hist[p.few][i + 1 < ns ? 0 : bucket(p, p.n - (ns - 1) * ks[p.few])], 1);
+        if (at >= (p.few ? a.max_few : a.max_items)) return;
+        int4* e = reinterpret_cast<int4*>((p.few ? few_list : list) + (int64_t)at * ATTN_ITEM_WORDS);
+        e[0] = make_int4(p.q0, p.row0, p.rows, p.off);
+        e[1] = make_int4(i * len, min(p.keys, (i + 1) * len), ns > 1 ? part + i * p.rows : -1, p.b);
+    };
+    for (int t0 = tid - lane; t0 < tiles; t0 += PLAN_THREADS) {
+        const int t = t0 + lane;
+        PlanTile p = {};
+        if (t < tiles) p = tile(t);
+        const int ns = p.rows > 0 ? splits(p) : 0;
+        if (ns == 1) put(p, 0, 1, -1);
+        // split tiles one after the other, the wave's lanes on their items and their rows to merge
+        for (unsigned long long left = __ballot(ns > 1); left; left &= left - 1) {
+            const int from = __builtin_ctzll(left);
+            PlanTile s;
+            s.b = __shfl(p.b, from);
+            s.q0 = __shfl(p.q0, from);
+            s.row0 = __shfl(p.row0, from);
+            s.rows = __shfl(p.rows, from);
+            s.off = __shfl(p.off, from);
+            s.keys = __shfl(p.keys, from);
+            s.unit = __shfl(p.unit, from);
+            s.n = __shfl(p.n, from);
+            s.few = __shfl((int)p.few, from) != 0;
+            const int n = __shfl(ns, from);
+            int part = 0, m = 0;
+            if (lane == 0) {
+                part = atomicAdd(&n_parts, n * s.rows);
+                m = atomicAdd(&n_merges, s.rows);
+            }
+            part = __shfl(part, 0);
+            m = __shfl(m, 0);
+            if (part + (int64_t)n * s.rows > a.max_part_rows || m + (int64_t)s.rows > a.max_merge_rows) continue;
+            // a row to merge: its token, its head of the group (bit 30: it sees no key), its first
+            // partial, and how many there are, s.rows apart
+            for (int r = lane; r < s.rows; r += 64) {
+                const int tok = (s.row0 + r) / a.G, g = s.row0 + r - tok * a.G;
+                merges[m + r] = make_int4(s.q0 + tok, g | (s.off + tok < 0 ? 1 << 30 : 0), part + r, n | s.rows << 16);
+            }
+            for (int i = lane; i < n; i += 64) put(s, i, n, part);
         }
     }
     __syncthreads();
     if (tid == 0) {
-        a.plan[ATTN_PLAN_ITEMS] = (int)min((int64_t)items, a.max_items);
+        a.plan[ATTN_PLAN_ITEMS] = (int)min((int64_t)items[0], a.max_items);
+        a.plan[ATTN_PLAN_FEW] = (int)min((int64_t)items[1], a.max_few);
         a.plan[ATTN_PLAN_MERGES] = (int)min((int64_t)n_merges, a.max_merge_rows);
     }
 }
@@ -204,7 +239,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) attn_plan_kernel(PlanArgs a) {
 
 extern "C" size_t oom_attn_plan_size(int T, int B, int heads, int kv_heads, int d) {
     if (T < 0 || B < 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || d < 1) return 0;
-    return (size_t)oom::attn_plan_dims(T, B, heads, kv_heads).words;
+    return (size_t)oom::attn_plan_dims(T, B, heads, kv_heads, d).words;
 }
 
 extern "C" int oom_attn_plan(const int32_t* cu_q, const int32_t* kv_lens, const int32_t* page_table, int max_pages,
@@ -225,7 +260,7 @@ extern "C" int oom_attn_plan(const int32_t* cu_q, const int32_t* kv_lens, const 
     OOM_REQUIRE(page_table || !slots, "oom_attn_plan: slots need a page_table");
     OOM_REQUIRE(plan && cu_q, "oom_attn_plan: null buffer");
     OOM_REQUIRE(aligned(plan, 16), "oom_attn_plan: plan must be 16-byte aligned");
-    const AttnPlanDims p = attn_plan_dims(T, B, heads, kv_heads);
+    const AttnPlanDims p = attn_plan_dims(T, B, heads, kv_heads, d);
     PlanArgs a;
     a.cu_q = cu_q;
     a.kv_lens = kv_lens;
@@ -237,7 +272,9 @@ extern "C" int oom_attn_plan(const int32_t* cu_q, const int32_t* kv_lens, const 
     a.T = T;
     a.G = heads / kv_heads;
     a.Hkv = kv_heads;
+    a.few_rows = attn_few_rows(d);
     a.max_items = p.items;
+    a.max_few = p.few_items;
     a.max_merge_rows = p.merge_rows;
     a.max_part_rows = p.part_rows;
     a.positions = positions;

@@ -223,11 +223,11 @@ struct Mx<16> {
 // output's own rounding; the sum l is that of the rounded p). TERMS 3: fp32 on either side: Q
 // and P enter as three exact bf16 terms each (hi + mid + lo), so products are exact and only
 // fp32 sums round.
-template <int D, int TERMS, int M>
+template <int D, int TERMS, int M, int KEYS = ATTN_KEYS>
 struct RowState {
     static constexpr int KD = 512 / M;    // dims (keys) a product sums over
     static constexpr int E = M * M / 64;  // elements of a result a lane
-    static constexpr int NS = 64 / M;     // results a tile of scores
+    static constexpr int NS = KEYS / M;   // results a tile of scores
     typedef typename Mx<M>::acc acc;
     tbf16x8 q[TERMS][D / KD];
     acc o[D / M];
@@ -240,8 +240,8 @@ struct RowState {
 template <int M>
 constexpr int score_key(int n, int i) { return M * n + (256 / M) * (i / 4) + i % 4; }
 
-template <int D, int TERMS, int M>
-__device__ __forceinline__ void rows_init(RowState<D, TERMS, M>& s, const TileArgs& a, const AttnItem& it, int h, int wrow,
+template <int D, int TERMS, int M, int KEYS>
+__device__ __forceinline__ void rows_init(RowState<D, TERMS, M, KEYS>& s, const TileArgs& a, const AttnItem& it, int h, int wrow,
                                           int lane) {
     const int r = wrow + lane % M, part = lane / M;
     s.live = r < it.rows;
@@ -289,14 +289,14 @@ __device__ __forceinline__ tbf16x8 t_finite8(tbf16x8 v) {
     return __builtin_bit_cast(tbf16x8, make_uint4(t_finite(w.x), t_finite(w.y), t_finite(w.z), t_finite(w.w)));
 }
 
-// One 64-key tile from LDS. MASKED: some key of the tile is hidden from some row, by a later position
+// Scores of one K tile from LDS. MASKED: some key of the tile is hidden from some row, by a later position
 // or past the item's keys (last: the last one that the lane's row sees). BAD_K, with three terms: K
 // holds infinities or NaN, which meet the first term alone; the others may be zero or of the
 // other sign. V holds none (the kernel takes them out).
-template <int D, int TERMS, int M, bool MASKED, bool BAD_K>
-__device__ __forceinline__ void tile_scores(RowState<D, TERMS, M>& s, const uint8_t* kt, int last, int lane) {
+template <bool MASKED, bool BAD_K, int D, int TERMS, int M, int KEYS>
+__device__ __forceinline__ void tile_scores(RowState<D, TERMS, M, KEYS>& s, const uint8_t* kt, int last, int lane) {
     typedef TileLay<D> L;
-    typedef RowState<D, TERMS, M> S;
+    typedef RowState<D, TERMS, M, KEYS> S;
     const int part = lane / M;
     const uint8_t* krow = kt + (lane % M) * L::ROWB;
     const int kx = L::kx(lane % M);  // rows M apart have the same
@@ -347,9 +347,9 @@ __device__ __forceinline__ float row_sum(float v) {
 
 // The running maximum; O and l rescaled where it grew enough. Returns what the tile's exponents
 // subtract.
-template <int D, int TERMS, int M>
-__device__ __forceinline__ float tile_maximum(RowState<D, TERMS, M>& s, float c) {
-    typedef RowState<D, TERMS, M> S;
+template <int D, int TERMS, int M, int KEYS>
+__device__ __forceinline__ float tile_maximum(RowState<D, TERMS, M, KEYS>& s, float c) {
+    typedef RowState<D, TERMS, M, KEYS> S;
     float mx = s.sc[0][0];
 #pragma unroll
     for (int n = 0; n < S::NS; n++)
@@ -378,16 +378,16 @@ __device__ __forceinline__ float tile_maximum(RowState<D, TERMS, M>& s, float c)
 }
 
 // The tile's weights p = 2^(s c - mb), their sum, and O += V^T P^T.
-template <int D, int TERMS, int M>
-__device__ __forceinline__ void tile_values(RowState<D, TERMS, M>& s, const uint8_t* vt, float c, float mb, int lane) {
+template <int D, int TERMS, int M, int KEYS>
+__device__ __forceinline__ void tile_values(RowState<D, TERMS, M, KEYS>& s, const uint8_t* vt, float c, float mb, int lane) {
     typedef TileLay<D> L;
-    typedef RowState<D, TERMS, M> S;
+    typedef RowState<D, TERMS, M, KEYS> S;
     const tbf16x2 ones = __builtin_bit_cast(tbf16x2, 0x3f803f80u);
     const int part = lane / M, r4 = (lane & 15) >> 2;
     const uint8_t* vrow = vt + (4 * part + r4) * L::ROWB + 8 * (lane & 1);
     const int vc = (M == 32 ? 2 * ((lane >> 4) & 1) : 0) + ((lane & 3) >> 1), vx = L::vx(4 * part + r4);
 #pragma unroll
-    for (int w = 0; w < 64 / S::KD; w++) {
+    for (int w = 0; w < KEYS / S::KD; w++) {
         // the lane's 8 keys of this product: two runs of four, 256 / M apart
         float p[8];
 #pragma unroll
@@ -429,11 +429,11 @@ __device__ __forceinline__ void tile_values(RowState<D, TERMS, M>& s, const uint
 
 // The infinities and NaN of a V tile to the rows that see their key: a hidden key has no part in a
 // row, whatever its value holds, and its weight of zero times an infinity would be NaN.
-template <int D, int TERMS, int M>
-__device__ __forceinline__ void tile_bad_values(RowState<D, TERMS, M>& s, const uint8_t* vt, int last, int lane) {
+template <int D, int TERMS, int M, int KEYS>
+__device__ __forceinline__ void tile_bad_values(RowState<D, TERMS, M, KEYS>& s, const uint8_t* vt, int last, int lane) {
     typedef TileLay<D> L;
     const int part = lane / M;
-    for (int key = 0; key < 64; key++) {
+    for (int key = 0; key < KEYS; key++) {
         if (!__any(key <= last)) break;
 #pragma unroll
         for (int d = 0; d < D / M; d++)
@@ -557,8 +557,8 @@ __global__ void __launch_bounds__(8192 / M, 2) attn_tile_kernel(TileArgs a) {
         const bool sees = has && (!MASKED || key0 <= pos_hi);  // uniform
         const int last = MASKED ? min(s.pos, it.k1 - 1) - key0 : 63;
         if (sees) {
-            if (TERMS > 1 && bad_lds[stage ? 2 : 0] != 0) tile_scores<D, TERMS, M, MASKED, true>(s, kt, last, lane);
-            else tile_scores<D, TERMS, M, MASKED, false>(s, kt, last, lane);
+            if (TERMS > 1 && bad_lds[stage ? 2 : 0] != 0) tile_scores<MASKED, true>(s, kt, last, lane);
+            else tile_scores<MASKED, false>(s, kt, last, lane);
         }
         const float mb = sees ? tile_maximum(s, c) : 0.0f;
         if ((MASKED || TERMS > 1) && bad_lds[stage ? 3 : 1] != 0) {  // uniform over the block; rare

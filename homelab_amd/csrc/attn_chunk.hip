@@ -81,7 +81,7 @@ template <int D>
 static int launch_chunk(const TileArgs& a, const AttnPlanDims& p, int B, int max_q, bool exact, hipStream_t st) {
     const int64_t most = (int64_t)max_q * a.G;
     if (most > attn_few_rows(D)) {
-        launch_tiles<D, true>(a, dim3((uint32_t)(p.items * a.Hkv)), exact, st);
+        launch_tiles<D, true>(a, p.items, exact, st);
         if (int rc = launched("oom_attn_chunk_paged")) return rc;
     }
     if (most <= attn_few_rows(D) || B > 1) {
@@ -127,7 +127,7 @@ extern "C" int oom_attn_chunk_paged(const void* q, int q_dtype, int64_t q_stride
     OOM_REQUIRE(aligned(q, 16) && aligned(k_pages, 16) && aligned(v_pages, 16) && aligned(out, 16) && aligned(plan, 16),
                 "oom_attn_chunk_paged: q, k_pages, v_pages, out and plan must be 16-byte aligned");
     const AttnPlanDims p = attn_plan_dims(T, B, heads, kv_heads, d);
-    OOM_REQUIRE(p.items * kv_heads < (1ll << 31), "oom_attn_chunk_paged: too many tiles of rows");
+    OOM_REQUIRE(p.items * kv_heads < (1ll << 30), "oom_attn_chunk_paged: too many tiles of rows");
     if (!ws || ws_bytes < oom_attn_chunk_paged_workspace_size(T, B, heads, kv_heads, d))
         return fail(OOM_ERR_WORKSPACE,
                     "oom_attn_chunk_paged: workspace smaller than oom_attn_chunk_paged_workspace_size()");

@@ -188,7 +188,7 @@ __device__ __forceinline__ void few_rows(const TileArgs& a, const AttnItem& it, 
 
 // Block i takes few-row item i / Hkv for KV head i % Hkv, with as many rows a wave as it needs.
 template <int D, int TERMS>
-__global__ void __launch_bounds__(64 * few_waves<D>(), 2) attn_few_kernel(TileArgs a, int64_t max_items) {
+__global__ void __launch_bounds__(64 * few_waves<D>(), D == 128 && TERMS == 3 ? 1 : 2) attn_few_kernel(TileArgs a, int64_t max_items) {
     __shared__ __align__(16) uint8_t lds[few_waves<D>() * 2 * FK * TileLay<D>::ROWB];
     __shared__ float mlds[few_waves<D>()][32], llds[few_waves<D>()][32];
     const int h = (int)(blockIdx.x % (uint32_t)a.Hkv), item = (int)(blockIdx.x / (uint32_t)a.Hkv);

@@ -8,8 +8,7 @@ namespace oom {
 
 template <int D>
 static int launch_prompt(const TileArgs& a, int64_t items, bool exact, hipStream_t st) {
-    const dim3 grid((uint32_t)(items * a.Hkv));
-    launch_tiles<D, false>(a, grid, exact, st);
+    launch_tiles<D, false>(a, items, exact, st);
     return launched("oom_attn_prompt");
 }
 
@@ -39,7 +38,7 @@ extern "C" int oom_attn_prompt(const void* q, int q_dtype, int64_t q_stride, con
     OOM_REQUIRE(aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && aligned(out, 16) && aligned(plan, 16),
                 "oom_attn_prompt: q, k, v, out and plan must be 16-byte aligned");
     const AttnPlanDims p = attn_plan_dims(T, B, heads, kv_heads, d);
-    OOM_REQUIRE(p.tiles * kv_heads < (1ll << 31), "oom_attn_prompt: too many tiles of rows");
+    OOM_REQUIRE(p.tiles * kv_heads < (1ll << 30), "oom_attn_prompt: too many tiles of rows");
     TileArgs a = {};
     a.q = q;
     a.q_stride = q_stride;

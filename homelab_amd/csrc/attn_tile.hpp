@@ -195,6 +195,11 @@ __device__ __forceinline__ uint32_t t_finite(uint32_t w) {
     return w & ~m;
 }
 
+__device__ __forceinline__ tbf16x8 t_finite8(tbf16x8 v) {
+    const uint4 w = __builtin_bit_cast(uint4, v);
+    return __builtin_bit_cast(tbf16x8, make_uint4(t_finite(w.x), t_finite(w.y), t_finite(w.z), t_finite(w.w)));
+}
+
 typedef float tf32x4 __attribute__((ext_vector_type(4)));
 
 // The matrix instruction of M rows: S^T tiles of M keys x M rows over 512 / M dims, O^T tiles of M
@@ -253,24 +258,31 @@ __device__ __forceinline__ void rows_init(RowState<D, TERMS, M, KEYS>& s, const 
     for (int d = 0; d < D / M; d++) s.o[d] = typename Mx<M>::acc{};
     constexpr int KD = 512 / M;
     const int64_t at = (int64_t)(it.q0 + (int)tok) * a.q_stride + (int64_t)(h * a.G + (int)g) * D + 8 * part;
-    if (a.q_dtype == OOM_BF16) {
+    if constexpr (TERMS == 1) {
         const uint16_t* p = reinterpret_cast<const uint16_t*>(a.q) + at;
 #pragma unroll
+        for (int c = 0; c < D / KD; c++)
+            s.q[0][c] = __builtin_bit_cast(tbf16x8, *reinterpret_cast<const uint4*>(p + KD * c));
+    } else {
+        const bool wide = a.q_dtype == OOM_F32;  // uniform
+        const uint8_t* p = reinterpret_cast<const uint8_t*>(a.q) + at * (wide ? 4 : 2);
+        uint4 raw[D / KD][2];
+#pragma unroll
         for (int c = 0; c < D / KD; c++) {
-            const uint4 v = *reinterpret_cast<const uint4*>(p + KD * c);
-            s.q[0][c] = __builtin_bit_cast(tbf16x8, v);
-            if constexpr (TERMS == 3)
-                s.q[1][c] = s.q[2][c] = __builtin_bit_cast(tbf16x8, make_uint4(0, 0, 0, 0));
+            raw[c][0] = *reinterpret_cast<const uint4*>(p + KD * c * (wide ? 4 : 2));
+            raw[c][1] = wide ? *reinterpret_cast<const uint4*>(p + KD * c * 4 + 16) : make_uint4(0, 0, 0, 0);
         }
-    } else if constexpr (TERMS == 3) {
-        const float* p = reinterpret_cast<const float*>(a.q) + at;
 #pragma unroll
         for (int c = 0; c < D / KD; c++) {
-            const float4 v0 = *reinterpret_cast<const float4*>(p + KD * c);
-            const float4 v1 = *reinterpret_cast<const float4*>(p + KD * c + 4);
-            float f[8] = {v0.x, v0.y, v0.z, v0.w, v1.x, v1.y, v1.z, v1.w};
+            const uint4 x = raw[c][0], y = raw[c][1];
+            const uint32_t n[8] = {x.x << 16, x.x & 0xffff0000u, x.y << 16, x.y & 0xffff0000u,
+                                   x.z << 16, x.z & 0xffff0000u, x.w << 16, x.w & 0xffff0000u};
+            const uint32_t f4[8] = {x.x, x.y, x.z, x.w, y.x, y.y, y.z, y.w};
+            float f[8];
 #pragma unroll
-            for (int t = 0; t < 3; t++) {
+            for (int e = 0; e < 8; e++) f[e] = __uint_as_float(wide ? f4[e] : n[e]);
+#pragma unroll
+            for (int t = 0; t < TERMS; t++) {
                 uint32_t w[4];
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
@@ -282,11 +294,6 @@ __device__ __forceinline__ void rows_init(RowState<D, TERMS, M, KEYS>& s, const 
             }
         }
     }
-}
-
-__device__ __forceinline__ tbf16x8 t_finite8(tbf16x8 v) {
-    const uint4 w = __builtin_bit_cast(uint4, v);
-    return __builtin_bit_cast(tbf16x8, make_uint4(t_finite(w.x), t_finite(w.y), t_finite(w.z), t_finite(w.w)));
 }
 
 // Scores of one K tile from LDS. MASKED: some key of the tile is hidden from some row, by a later position
@@ -301,11 +308,11 @@ __device__ __forceinline__ void tile_scores(RowState<D, TERMS, M, KEYS>& s, cons
     const uint8_t* krow = kt + (lane % M) * L::ROWB;
     const int kx = L::kx(lane % M);  // rows M apart have the same
 #pragma unroll
-    for (int n = 0; n < S::NS; n++) {
-        s.sc[n] = typename S::acc{};
+    for (int st = 0; st < D / S::KD; st++) {
+        const int chunk = (S::KD / 8 * st + part) ^ kx;
 #pragma unroll
-        for (int st = 0; st < D / S::KD; st++) {
-            const int chunk = (S::KD / 8 * st + part) ^ kx;
+        for (int n = 0; n < S::NS; n++) {
+            if (st == 0) s.sc[n] = typename S::acc{};
             const uint4 kv = *reinterpret_cast<const uint4*>(krow + M * n * L::ROWB + 16 * chunk);
             const tbf16x8 ka = __builtin_bit_cast(tbf16x8, kv);
             if constexpr (TERMS > 1) {
@@ -489,26 +496,31 @@ __device__ __forceinline__ void rows_store(RowState<D, TERMS, M>& s, const TileA
         }
 }
 
-// Blocks of 128 rows, M a wave; block i takes item i / Hkv for KV head i % Hkv (consecutive blocks
-// run on different XCDs, so with 8 KV heads each L2 holds one head's K and V).
+// NW waves of M rows a block: a whole tile of 128 rows, or part of one; block i takes part i / Hkv
+// for KV head i % Hkv (consecutive blocks run on different XCDs, so with 8 KV heads each L2 holds
+// one head's K and V).
 // K and V tiles go through LDS in two stages, one barrier a tile: past it, every wave has done
 // with the stage that the next tile's loads now fill, and those have a whole tile to arrive.
 // Two blocks a CU (d up to 128) or two waves a SIMD take turns on the matrix cores and the
 // vector units.
-template <int D, int TERMS, int M, bool PAGED>
-__global__ void __launch_bounds__(8192 / M, 2) attn_tile_kernel(TileArgs a) {
+template <int D, int TERMS, int M, int NW, bool PAGED>
+__global__ void __launch_bounds__(64 * NW, 2) attn_tile_kernel(TileArgs a) {
     typedef TileLay<D> L;
-    constexpr int NW = 128 / M;
+    constexpr int ROWS = NW * M, PARTS = ATTN_ROWS / ROWS;
     __shared__ __align__(16) uint8_t tiles[4 * L::BYTES];  // stage 0: K, V; stage 1: K, V
     __shared__ uint32_t bad_lds[4];                        // per stage: K, V hold infinities or NaN
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = (int)(blockIdx.x % (uint32_t)a.Hkv), item = (int)(blockIdx.x / (uint32_t)a.Hkv);
-    const AttnItem it = reinterpret_cast<const AttnItem*>(a.plan + ATTN_PLAN_HEAD)[item];
-    if (item >= a.plan[ATTN_PLAN_ITEMS]) return;
-    const int wrow = M * wave;
+    const int h = (int)(blockIdx.x % (uint32_t)a.Hkv), block = (int)(blockIdx.x / (uint32_t)a.Hkv);
+    const int item = block / PARTS, row_b = block % PARTS * ROWS;  // the block's first row of the tile
+    AttnItem it = reinterpret_cast<const AttnItem*>(a.plan + ATTN_PLAN_HEAD)[item];
+    if (item >= a.plan[ATTN_PLAN_ITEMS] || row_b >= it.rows) return;
+    const int wrow = row_b + M * wave;
     const bool has = wrow < it.rows;  // uniform
     const float c = a.scale * 1.44269504088896340736f;
+    // no row of the block sees keys past its last row's position
+    if constexpr (PARTS > 1)
+        it.k1 = min(it.k1, it.off + 1 + (int)((uint32_t)(it.row0 + min(row_b + ROWS, it.rows) - 1) / (uint32_t)a.G));
     TileSrc<D, NW, PAGED> src;
     src.init(a, it, h, lane, wave);
     if (threadIdx.x < 4) bad_lds[threadIdx.x] = 0;
@@ -520,7 +532,7 @@ __global__ void __launch_bounds__(8192 / M, 2) attn_tile_kernel(TileArgs a) {
     __syncthreads();  // bad_lds is cleared
     // the wave's last position; the tiles that every row of the block sees whole come first
     const int pos_hi = it.off + (int)((uint32_t)(it.row0 + min(wrow + M - 1, it.rows - 1)) / (uint32_t)a.G);
-    const int block_lo = it.off + (int)((uint32_t)it.row0 / (uint32_t)a.G);
+    const int block_lo = it.off + (int)((uint32_t)(it.row0 + row_b) / (uint32_t)a.G);
     const int whole = it.k0 + (max(0, min(it.k1, block_lo + 1) - it.k0) & ~63);
     int key0 = it.k0;
     uint32_t stage = 0;
@@ -580,15 +592,17 @@ __global__ void __launch_bounds__(8192 / M, 2) attn_tile_kernel(TileArgs a) {
 }
 
 // Rows a wave: 32 up to d 128 in one term; 16 for three terms and for d 256, whose Q and O of 32 rows
-// leave no registers for a second wave on the SIMD.
-template <int D, int TERMS>
-constexpr int tile_m() { return D <= 128 && TERMS == 1 ? 32 : 16; }
-
+// leave no registers for a second wave on the SIMD. Waves a block: a tile's rows, but half of
+// them for three terms up to d 128, so that two blocks fit a CU and do not wait at the same
+// barriers (LDS holds one block at d 256).
 template <int D, bool PAGED>
-void launch_tiles(const TileArgs& a, dim3 grid, bool exact, hipStream_t st) {
-    constexpr int M1 = tile_m<D, 1>(), M3 = tile_m<D, 3>();
-    if (exact) hipLaunchKernelGGL((attn_tile_kernel<D, 3, M3, PAGED>), grid, dim3(8192 / M3), 0, st, a);
-    else hipLaunchKernelGGL((attn_tile_kernel<D, 1, M1, PAGED>), grid, dim3(8192 / M1), 0, st, a);
+void launch_tiles(const TileArgs& a, int64_t items, bool exact, hipStream_t st) {
+    constexpr int M1 = D <= 128 ? 32 : 16, NW1 = ATTN_ROWS / M1, NW3 = D <= 128 ? 4 : 8;
+    const int64_t n = items * a.Hkv;
+    if (exact)
+        hipLaunchKernelGGL((attn_tile_kernel<D, 3, 16, NW3, PAGED>), dim3((uint32_t)(n * (8 / NW3))), dim3(64 * NW3), 0, st, a);
+    else
+        hipLaunchKernelGGL((attn_tile_kernel<D, 1, M1, NW1, PAGED>), dim3((uint32_t)n), dim3(64 * NW1), 0, st, a);
 }
 
 }  // namespace oom

@@ -8,11 +8,11 @@ namespace oom {
 
 // The merge of split rows: a wave a (row, KV head), in turn over all of them. The parts' maxima give
 // their weights e^((m_p - M) scale); out = sum_p w_p O_p / sum_p w_p l_p. A load takes the row of
-// 256 / d parts, 16 bytes a lane; the first 16 loads' parts are on their way before the weights
+// 256 / d parts, 16 bytes a lane; the first 8 loads' parts are on their way before the weights
 // are known, so a row takes two round trips, its entry and then everything.
 template <int D>
 __global__ void __launch_bounds__(256) attn_rows_merge_kernel(TileArgs a, const int4* rows) {
-    constexpr int LPP = D / 4, PP = 64 / LPP, EARLY = 16;  // lanes a part, parts a load, loads at once
+    constexpr int LPP = D / 4, PP = 64 / LPP, EARLY = 8;  // lanes a part, parts a load, loads at once
     const int lane = threadIdx.x & 63, sub = lane / LPP, col = lane % LPP * 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
     const int64_t all = (int64_t)a.plan[ATTN_PLAN_MERGES] * a.Hkv;

@@ -40,21 +40,18 @@ __device__ __forceinline__ void few_rows(const TileArgs& a, const AttnItem& it, 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const float c = a.scale * 1.44269504088896340736f;
     const int32_t* const table = a.table + (size_t)it.seq * a.max_pages;
-    const int p16 = a.page_size / 16;
-    const int64_t page_bytes = (int64_t)a.page_size * a.Hkv * D * 2;
     const uint8_t* const kb = (const uint8_t*)a.k + (int64_t)h * a.page_size * D * 2;
     const uint8_t* const vb = (const uint8_t*)a.v + (int64_t)h * a.page_size * D * 2;
     const uint8_t* const kt = lds + wave * 2 * TB;
     uint8_t* const vt = lds + wave * 2 * TB + TB;
     const uint32_t k_at = (uint32_t)(uintptr_t)(t_lds_t)lds + wave * 2 * TB, v_at = k_at + TB;
-    // tile t of the wave starts at key0(t); its run x's page is in lane 2 t + x (t modulo 32)
+    // tile t of the wave starts at key0(t); its run x's place is in lane 2 t + x (t modulo 32)
     const auto key0 = [&](int t) { return it.k0 + FK * (wave + NW * t); };
     const int left = it.k1 - key0(0);
     const int n = left > 0 ? (left + FK * NW - 1) / (FK * NW) : 0;  // the wave's tiles
-    int pages = -1;
-    const auto find_pages = [&](int t0) {
-        const int key = key0(t0 + lane / PIECES) + 16 * (lane % PIECES);
-        pages = key < it.k1 ? table[(uint32_t)key / 16 / (uint32_t)p16] : -1;
+    int64_t found = -1;
+    const auto find_places = [&](int t0) {
+        found = page_offset(a, table, key0(t0 + lane / PIECES) + 16 * (lane % PIECES), it.k1, L::ROWB);
     };
     uint32_t ko[NI], vo[NI];
 #pragma unroll
@@ -67,10 +64,10 @@ __device__ __forceinline__ void few_rows(const TileArgs& a, const AttnItem& it, 
     const auto load = [&](int t, const uint8_t* base, const uint32_t (&off)[NI], uint32_t to) {
 #pragma unroll
         for (int x = 0; x < PIECES; x++) {
-            const int key = key0(t) + 16 * x, page = __builtin_amdgcn_readlane(pages, (PIECES * t + x) & 63);
-            const bool ok = page >= 0 && page < a.n_pages;
-            const uint32_t sub = (uint32_t)key / 16;
-            const uint8_t* at = base + ((ok ? page : 0) * page_bytes + (int64_t)(sub % (uint32_t)p16) * 16 * L::ROWB);
+            const int key = key0(t) + 16 * x;
+            const int64_t place = lane_value(found, (PIECES * t + x) & 63);
+            const bool ok = place >= 0;
+            const uint8_t* at = base + place;
             if (ok && key + 16 <= it.k1) {  // uniform
 #pragma unroll
                 for (int i = 0; i < NI; i++) t_load_lds(at, off[i], to + x * 16 * L::ROWB + i * 1024);
@@ -83,7 +80,7 @@ __device__ __forceinline__ void few_rows(const TileArgs& a, const AttnItem& it, 
             }
         }
     };
-    if (n > 0) find_pages(0);
+    if (n > 0) find_places(0);
     RowState<D, TERMS, M, FK> s;
     rows_init(s, a, it, h, 0, lane);
     t_wait_loads();  // the compiler's own loads are done: from here on the count is the tiles'
@@ -109,7 +106,7 @@ __device__ __forceinline__ void few_rows(const TileArgs& a, const AttnItem& it, 
         if (TERMS > 1 && look(kt)) tile_scores<MASKED, true>(s, kt, last, lane);
         else tile_scores<MASKED, false>(s, kt, last, lane);
         if (more && (t + 1) % (64 / PIECES) == 0) {
-            find_pages(t + 1);
+            find_places(t + 1);
             t_wait_loads();
         }
         if (more) load(t + 1, kb, ko, k_at);

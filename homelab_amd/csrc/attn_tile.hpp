@@ -115,60 +115,78 @@ __device__ __forceinline__ void t_wait_loads() {
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
+// Where a run of keys lies in its page: byte offset from the head's first row of page 0, or -1 (a bad
+// page, or past the item's keys).
+__device__ __forceinline__ int64_t page_offset(const TileArgs& a, const int32_t* table, int key, int k1, int row_bytes) {
+    if (key >= k1) return -1;
+    const uint32_t pi = (uint32_t)key / (uint32_t)a.page_size;
+    const int page = table[pi];
+    if (page < 0 || page >= a.n_pages) return -1;
+    return ((int64_t)page * a.Hkv * a.page_size + (key - (int)pi * a.page_size)) * row_bytes;
+}
+__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
+    const uint32_t lo = __builtin_amdgcn_readlane((int)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+    return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 // Loads of one 64-key tile: wave w of NW takes 64 / NW rows of K and of V, which lie in one page.
+// Over pages, lane i holds the place of the wave's rows of tile i (modulo 64): looked up a tile at a
+// time, each tile waited for its page index before its loads could go out (100 tokens over 1300
+// keys 20.6 us, so 14.9).
 template <int D, int NW, bool PAGED>
 struct TileSrc {
     typedef TileLay<D> L;
     static constexpr int WR = 64 / NW, NI = WR / L::RPI;  // rows and instructions a wave
     static_assert(NI >= 1 && WR <= 16 && 16 % WR == 0, "whole instructions, one 16-key run");
-    const uint16_t *k, *v;
-    int64_t ks, vs;  // elements between rows
+    const uint8_t *k, *v;
+    int64_t ks, vs;  // bytes between rows
     const int32_t* table;
-    int n_pages, p16, k1;
-    int64_t page_elems;
+    int first, k1;  // the wave's first key; the item's end
+    int64_t places;
     uint32_t ko[NI], vo[NI];  // byte offsets of this lane from the wave's first row
 
     __device__ __forceinline__ void init(const TileArgs& a, const AttnItem& it, int h, int lane, int wave) {
         k1 = it.k1;
+        first = it.k0 + WR * wave;
+        k = reinterpret_cast<const uint8_t*>(a.k);
+        v = reinterpret_cast<const uint8_t*>(a.v);
         if constexpr (PAGED) {
-            ks = vs = D;
+            ks = vs = L::ROWB;
             table = a.table + (size_t)it.seq * a.max_pages;
-            n_pages = a.n_pages;
-            p16 = a.page_size / 16;
-            page_elems = (int64_t)a.page_size * a.Hkv * D;
-            k = a.k + (int64_t)h * a.page_size * D;
-            v = a.v + (int64_t)h * a.page_size * D;
+            k += (int64_t)h * a.page_size * L::ROWB;
+            v += (int64_t)h * a.page_size * L::ROWB;
         } else {
-            ks = a.k_stride;
-            vs = a.v_stride;
-            k = a.k + (int64_t)it.q0 * ks + h * D;
-            v = a.v + (int64_t)it.q0 * vs + h * D;
+            ks = 2 * a.k_stride;
+            vs = 2 * a.v_stride;
+            k += (int64_t)it.q0 * ks + h * L::ROWB;
+            v += (int64_t)it.q0 * vs + h * L::ROWB;
         }
 #pragma unroll
         for (int n = 0; n < NI; n++) {
             const int r = n * L::RPI + lane / L::C, c = lane % L::C;
-            ko[n] = (uint32_t)(r * ks * 2) + 16 * (c ^ L::kx(WR * wave + r));
-            vo[n] = (uint32_t)(r * vs * 2) + 16 * (c ^ L::vx(WR * wave + r));
+            ko[n] = (uint32_t)(r * ks) + 16 * (c ^ L::kx(WR * wave + r));
+            vo[n] = (uint32_t)(r * vs) + 16 * (c ^ L::vx(WR * wave + r));
         }
     }
 
-    // The wave's rows from key `key` (a multiple of 64 / NW) on into its places kt and vt (LDS byte
-    // addresses of its first row in the K and the V tile).
-    __device__ __forceinline__ void load(int key, int lane, uint32_t kt, uint32_t vt) const {
-        int64_t kat = 0, vat = 0;
+    // The wave's rows of tile t into its places kt and vt (LDS byte addresses of its first row in the
+    // K and the V tile).
+    __device__ __forceinline__ void load(const TileArgs& a, int t, int lane, uint32_t kt, uint32_t vt) {
+        const int key = first + 64 * t;
+        int64_t kat, vat;
         bool ok = key < k1;
         if constexpr (PAGED) {
-            if (ok) {
-                const uint32_t sub = (uint32_t)key / 16, pi = sub / (uint32_t)p16, si = sub - pi * p16;
-                const int page = table[pi];
-                ok = page >= 0 && page < n_pages;
-                kat = vat = (ok ? page : 0) * page_elems + (int64_t)(si * 16 + key % 16) * D;
+            if (t % 64 == 0) {
+                places = page_offset(a, table, key + 64 * lane, k1, L::ROWB);
+                __builtin_amdgcn_s_waitcnt(0);
             }
+            kat = vat = lane_value(places, t % 64);
+            ok = kat >= 0;
         } else {
             kat = key * ks;
             vat = key * vs;
         }
-        const uint16_t *kb = k + kat, *vb = v + vat;
+        const uint8_t *kb = k + kat, *vb = v + vat;
         if (ok && key + WR <= k1) {  // uniform
 #pragma unroll
             for (int n = 0; n < NI; n++) t_load_lds(kb, ko[n], kt + n * 1024);
@@ -180,8 +198,8 @@ struct TileSrc {
 #pragma unroll
         for (int n = 0; n < NI; n++) {
             const bool in = ok && key + n * L::RPI + lane / L::C < k1;
-            t_load_lds(in ? (const uint8_t*)kb + ko[n] : z, kt + n * 1024);
-            t_load_lds(in ? (const uint8_t*)vb + vo[n] : z, vt + n * 1024);
+            t_load_lds(in ? kb + ko[n] : z, kt + n * 1024);
+            t_load_lds(in ? vb + vo[n] : z, vt + n * 1024);
         }
     }
 };
@@ -460,40 +478,61 @@ __device__ __forceinline__ void tile_bad_values(RowState<D, TERMS, M, KEYS>& s, 
     }
 }
 
+// The token row and the head of the group of packed row r of the sequence.
+__device__ __forceinline__ int64_t row_at(const TileArgs& a, const AttnItem& it, int h, int D, int r) {
+    const uint32_t row = (uint32_t)(it.row0 + r), tok = row / (uint32_t)a.G, g = row - tok * a.G;
+    return (int64_t)(it.q0 + (int)tok) * a.out_stride + (int64_t)(h * a.G + (int)g) * D;
+}
+
 // out = O / l of the wave's rows, or their partial (O, m, l) for the merge. A row that sees no key
-// gives zeros.
+// gives zeros. Lanes hold columns of rows: they go through LDS (the wave's share of the tiles' places,
+// which no wave reads any more) so that a store covers whole rows, 1 KB at a time; chunks of 16
+// bytes are permuted within a row against bank conflicts. (Stored from the registers, 8 or 16
+// bytes a row and instruction: 2 % slower on short prompts.)
 template <int D, int TERMS, int M>
 __device__ __forceinline__ void rows_store(RowState<D, TERMS, M>& s, const TileArgs& a, const AttnItem& it, int h, int wrow,
-                                           int lane) {
-    const int r = wrow + lane % M, part = lane / M;
+                                           int lane, uint8_t* lds) {
+    const int r = lane % M, part = lane / M;
     s.l = row_sum<M>(s.l);
-    if (!s.live) return;
-    if (it.part >= 0) {
-        const int64_t pr = (int64_t)h * a.part_rows + it.part + r;
-        if (part == 0) *reinterpret_cast<float2*>(a.part_ml + 2 * pr) = make_float2(s.m, s.l);
-#pragma unroll
-        for (int d = 0; d < D / M; d++)
-#pragma unroll
-            for (int e = 0; e < M * M / 256; e++)
-                *reinterpret_cast<float4*>(a.part_acc + pr * D + M * d + 256 / M * e + 4 * part) =
-                    make_float4(s.o[d][4 * e], s.o[d][4 * e + 1], s.o[d][4 * e + 2], s.o[d][4 * e + 3]);
-        return;
-    }
-    const float inv = s.pos < 0 ? 0.0f : 1.0f / s.l;
-    const uint32_t row = (uint32_t)(it.row0 + r), tok = row / (uint32_t)a.G, g = row - tok * a.G;
-    const int64_t at = (int64_t)(it.q0 + (int)tok) * a.out_stride + (int64_t)(h * a.G + (int)g) * D + 4 * part;
+    const bool wide = it.part >= 0 || a.out_dtype == OOM_F32;  // uniform
+    const int64_t pr = (int64_t)h * a.part_rows + it.part + wrow;
+    if (it.part >= 0 && part == 0 && s.live) *reinterpret_cast<float2*>(a.part_ml + 2 * (pr + r)) = make_float2(s.m, s.l);
+    const float f = it.part >= 0 ? 1.0f : s.pos < 0 ? 0.0f : 1.0f / s.l;
 #pragma unroll
     for (int d = 0; d < D / M; d++)
 #pragma unroll
         for (int e = 0; e < M * M / 256; e++) {
-            const float x0 = s.o[d][4 * e] * inv, x1 = s.o[d][4 * e + 1] * inv, x2 = s.o[d][4 * e + 2] * inv,
-                        x3 = s.o[d][4 * e + 3] * inv;
-            const int64_t i = at + M * d + 256 / M * e;
-            if (a.out_dtype == OOM_BF16)
-                *reinterpret_cast<uint2*>(reinterpret_cast<uint16_t*>(a.out) + i) = make_uint2(t_pack(x0, x1), t_pack(x2, x3));
+            const float x0 = s.o[d][4 * e] * f, x1 = s.o[d][4 * e + 1] * f, x2 = s.o[d][4 * e + 2] * f,
+                        x3 = s.o[d][4 * e + 3] * f;
+            const int dim = M * d + 256 / M * e + 4 * part;
+            if (wide)
+                *reinterpret_cast<float4*>(lds + r * D * 4 + 16 * ((dim / 4) ^ (r & 15))) = make_float4(x0, x1, x2, x3);
             else
-                *reinterpret_cast<float4*>(reinterpret_cast<float*>(a.out) + i) = make_float4(x0, x1, x2, x3);
+                *reinterpret_cast<uint2*>(lds + r * D * 2 + 16 * ((dim / 8) ^ (r & (D / 8 - 1) & 15)) + 2 * (dim & 7)) =
+                    make_uint2(t_pack(x0, x1), t_pack(x2, x3));
         }
+    wave_lds_order();
+    if (wide) {
+        constexpr int C = D / 4;  // chunks a row
+#pragma unroll
+        for (int i = 0; i < M * C / 64; i++) {
+            const int row = (64 * i + lane) / C, ch = (64 * i + lane) % C;
+            if (wrow + row >= it.rows) continue;
+            const float4 v = *reinterpret_cast<const float4*>(lds + row * D * 4 + 16 * (ch ^ (row & 15)));
+            float* to = it.part >= 0 ? a.part_acc + (pr + row) * D
+                                     : reinterpret_cast<float*>(a.out) + row_at(a, it, h, D, wrow + row);
+            *reinterpret_cast<float4*>(to + 4 * ch) = v;
+        }
+    } else {
+        constexpr int C = D / 8;
+#pragma unroll
+        for (int i = 0; i < M * C / 64; i++) {
+            const int row = (64 * i + lane) / C, ch = (64 * i + lane) % C;
+            if (wrow + row >= it.rows) continue;
+            const uint4 v = *reinterpret_cast<const uint4*>(lds + row * D * 2 + 16 * (ch ^ (row & (C - 1) & 15)));
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + row_at(a, it, h, D, wrow + row) + 8 * ch) = v;
+        }
+    }
 }
 
 // NW waves of M rows a block: a whole tile of 128 rows, or part of one; block i takes part i / Hkv
@@ -525,8 +564,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_tile_kernel(TileArgs a) {
     src.init(a, it, h, lane, wave);
     if (threadIdx.x < 4) bad_lds[threadIdx.x] = 0;
     const uint32_t mine = (uint32_t)(uintptr_t)(t_lds_t)tiles + wave * (L::BYTES / NW);  // LDS address of the wave's rows
-    constexpr int WR = 64 / NW;                                                       // rows a wave loads
-    if (it.k0 < it.k1) src.load(it.k0 + WR * wave, lane, mine, mine + L::BYTES);
+    if (it.k0 < it.k1) src.load(a, 0, lane, mine, mine + L::BYTES);
     RowState<D, TERMS, M> s;
     rows_init(s, a, it, h, wrow, lane);
     __syncthreads();  // bad_lds is cleared
@@ -564,7 +602,7 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_tile_kernel(TileArgs a) {
         t_barrier();
         if (key0 + 64 < it.k1) {
             const uint32_t to = mine + (stage ^ (2 * L::BYTES));
-            src.load(key0 + 64 + WR * wave, lane, to, to + L::BYTES);
+            src.load(a, (key0 + 64 - it.k0) / 64, lane, to, to + L::BYTES);
         }
         const bool sees = has && (!MASKED || key0 <= pos_hi);  // uniform
         const int last = MASKED ? min(s.pos, it.k1 - 1) - key0 : 63;
@@ -588,7 +626,9 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_tile_kernel(TileArgs a) {
     };
     for (; key0 < whole; key0 += 64, stage ^= 2 * L::BYTES) step(std::false_type{});
     for (; key0 < it.k1; key0 += 64, stage ^= 2 * L::BYTES) step(std::true_type{});
-    if (has) rows_store(s, a, it, h, wrow, lane);
+    __syncthreads();  // every wave is done with the tiles
+    static_assert(4 * L::BYTES >= NW * M * D * 4, "the rows fit the tiles' places");
+    if (has) rows_store(s, a, it, h, wrow, lane, tiles + wave * (M * D * 4));
 }
 
 // Rows a wave: 32 up to d 128 in one term; 16 for three terms and for d 256, whose Q and O of 32 rows

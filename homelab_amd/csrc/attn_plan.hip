@@ -12,7 +12,7 @@ struct PlanArgs {
     const int32_t* cu_q;
     const int32_t* kv_lens;  // null: prompts, whose keys are their own tokens
     const int32_t* table;
-    int max_pages, n_pages, page_size, B, T, G, Hkv, few_rows;
+    int max_pages, n_pages, page_size, B, T, G, Hkv, few_rows, split_blocks;
     int64_t max_items, max_few, max_merge_rows, max_part_rows;
     int32_t* positions;
     int64_t* slots;
@@ -151,13 +151,31 @@ __global__ void __launch_bounds__(PLAN_THREADS) attn_plan_kernel(PlanArgs a) {
         atomicMax(&longest[p.few], p.n);
     }
     __syncthreads();
-    // units a split. Prompts are not split: their rows alone fill the chip, or their keys are few
+    // Units a split. Prompts are not split: their rows alone fill the chip, or their keys are few. Else
+    // the work's even share a block, or up to a quarter more where that keeps the splits to as many
+    // blocks as run at once, so that no few of them make a second round (512 tokens over 16 Ki
+    // keys, d 128: 284 us with the share, 275 so; with no bound on the share, 3 x 300 tokens over
+    // up to 3000 keys at d 256 took 104 us, not 71).
     int ks[2] = {longest[0], longest[1]};
     if (a.kv_lens) {
-        const unsigned long long k0 = (work[0] * a.Hkv + ATTN_SPLIT_BLOCKS - 1) / ATTN_SPLIT_BLOCKS;
-        const unsigned long long k1 = (work[1] * a.Hkv + ATTN_FEW_BLOCKS - 1) / ATTN_FEW_BLOCKS;
-        ks[0] = (int)min((unsigned long long)longest[0], max(k0, 4ull));
-        ks[1] = (int)min((unsigned long long)longest[1], max(k1, 1ull));
+        PlanTile p = {};
+        if (tid < tiles) p = tile(tid);
+        for (int f = 0; f < 2; f++) {
+            const int slots = f ? ATTN_FEW_BLOCKS : a.split_blocks;
+            const unsigned long long even = (work[f] * a.Hkv + slots - 1) / slots;
+            const int share = (int)min((unsigned long long)longest[f], max(even, f ? 1ull : 4ull));
+            ks[f] = share;
+            // (more tiles than threads are more than the blocks: no search)
+            if (tiles > PLAN_THREADS) continue;
+            for (int k = share; k <= share + share / 4 && k < longest[f]; k += max(1, share / 16)) {
+                int all;
+                block_scan(p.rows > 0 && p.few == (f == 1) ? (p.n + k - 1) / k : 0, tmp, all);
+                if ((int64_t)all * a.Hkv <= slots) {
+                    ks[f] = k;
+                    break;
+                }
+            }
+        }
     }
     const auto splits = [&](const PlanTile& p) { return max(1, (p.n + ks[p.few] - 1) / ks[p.few]); };
     const auto bucket = [&](const PlanTile& p, int n) {
@@ -273,6 +291,7 @@ extern "C" int oom_attn_plan(const int32_t* cu_q, const int32_t* kv_lens, const 
     a.G = heads / kv_heads;
     a.Hkv = kv_heads;
     a.few_rows = attn_few_rows(d);
+    a.split_blocks = attn_split_blocks(d);
     a.max_items = p.items;
     a.max_few = p.few_items;
     a.max_merge_rows = p.merge_rows;

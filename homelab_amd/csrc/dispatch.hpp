@@ -299,14 +299,18 @@ inline int attn_pairs(int kv_len, int heads, int kv_heads, int d, size_t ws_byte
 constexpr int ATTN_ROWS = 128;        // packed rows (token, query head of a group) a tile
 constexpr int ATTN_KEYS = 64;         // keys a tile
 constexpr int ATTN_FEW_KEYS = 128;    // keys that a block of attn_few.hpp takes them in units of
-constexpr int ATTN_SPLIT_BLOCKS = 512;  // blocks that a batch's keys are split for: two a CU,
-constexpr int ATTN_FEW_BLOCKS = 256;    // and one a CU for the few-row sequences
+constexpr int ATTN_FEW_BLOCKS = 256;  // blocks that the few-row sequences' keys are split for, one a CU
 constexpr int ATTN_MAXB = 4096;       // sequences of a plan
 constexpr int ATTN_MAX_KEYS = 1 << 27;  // keys of a sequence
 
 // A sequence of at most so many packed rows over a paged cache is one tile of attn_few.hpp, whose
 // waves hold all of them: at d 256, Q and O of 32 rows would not fit a wave's registers.
 constexpr int attn_few_rows(int d) { return d == 256 ? 16 : 32; }
+
+// Blocks that the other sequences' keys are split for: as many as the chip holds at once, two a CU,
+// but one at d 256, whose tiles fill a CU's LDS (128 tokens over 8000 keys at 24/2 heads: 47 us
+// with 256 blocks, 58 with 512; at d 128, 64/8 heads, 512 over 16 Ki keys: 350 with 256, 300 with 512).
+constexpr int attn_split_blocks(int d) { return d == 256 ? 256 : 512; }
 
 // A plan in i32 words: ATTN_PLAN_HEAD words of counts, then the items, the few-row sequences' items,
 // and the rows to merge.
@@ -315,9 +319,9 @@ constexpr int ATTN_ITEM_WORDS = 8, ATTN_MERGE_WORDS = 4;
 constexpr int ATTN_PLAN_ITEMS = 0, ATTN_PLAN_FEW = 1, ATTN_PLAN_MERGES = 2;  // head words: how many of each
 
 // The plan's bounds, from sizes that the host knows. Tiles of sequence b: ceil(n_b G / 128), so at
-// most T G / 128 + B in all. With W key tiles over them and splits of ks = ceil(W Hkv / 512),
-// the items number at most tiles + W / ks and the tiles that are split at all (more than ks
-// key tiles) at most W / ks <= ceil(512 / Hkv); their parts at most twice that. The few-row
+// most T G / 128 + B in all. With W key tiles over them and splits of ks = ceil(W Hkv /
+// blocks), the items number at most tiles + W / ks and the tiles that are split at all (more than ks
+// key tiles) at most W / ks <= ceil(blocks / Hkv); their parts at most twice that. The few-row
 // sequences alike, one tile each.
 struct AttnPlanDims {
     int64_t tiles, items, few_items, merge_rows, part_rows, words;
@@ -325,7 +329,7 @@ struct AttnPlanDims {
 inline AttnPlanDims attn_plan_dims(int64_t T, int64_t B, int heads, int kv_heads, int d) {
     AttnPlanDims p;
     const int64_t rows = T * (heads / kv_heads);
-    const int64_t split = cdiv(ATTN_SPLIT_BLOCKS, kv_heads), few = cdiv(ATTN_FEW_BLOCKS, kv_heads);
+    const int64_t split = cdiv(attn_split_blocks(d), kv_heads), few = cdiv(ATTN_FEW_BLOCKS, kv_heads);
     const int64_t tile_rows = std::min<int64_t>(ATTN_ROWS, rows), few_rows = std::min<int64_t>(attn_few_rows(d), rows);
     p.tiles = rows / ATTN_ROWS + B;
     p.items = p.tiles + split;

@@ -15,7 +15,7 @@ __global__ void __launch_bounds__(256) attn_rows_merge_kernel(TileArgs a, const 
     constexpr int LPP = D / 4, PP = 64 / LPP, EARLY = 8;  // lanes a part, parts a load, loads at once
     const int lane = threadIdx.x & 63, sub = lane / LPP, col = lane % LPP * 4;
     const int wave = __builtin_amdgcn_readfirstlane((int)(blockIdx.x * 4 + (threadIdx.x >> 6)));
-    const int64_t all = (int64_t)a.plan[ATTN_PLAN_MERGES] * a.Hkv;
+    const int64_t all = a.plan[ATTN_PLAN_SIGN] == a.plan_sign ? (int64_t)a.plan[ATTN_PLAN_MERGES] * a.Hkv : 0;
     const float c = a.scale * 1.44269504088896340736f;
     for (int64_t i = wave; i < all; i += gridDim.x * 4) {
         const int h = (int)(i % a.Hkv);
@@ -50,7 +50,7 @@ __global__ void __launch_bounds__(256) attn_rows_merge_kernel(TileArgs a, const 
                 for (int j = 0; j < EARLY; j++) {
                     const int p = q0 + PP * j + sub;
                     const float wj = __shfl(w, p & 63);
-                    if (p < 64 && p0 + p < n) {
+                    if (p < 64 && p0 + p < n && wj != 0.0f) {  // (an empty partial's O is not written)
                         A[0] = fmaf(v[j].x, wj, A[0]);
                         A[1] = fmaf(v[j].y, wj, A[1]);
                         A[2] = fmaf(v[j].z, wj, A[2]);
@@ -146,6 +146,7 @@ extern "C" int oom_attn_chunk_paged(const void* q, int q_dtype, int64_t q_stride
     a.n_pages = n_pages;
     a.page_size = page_size;
     a.plan = plan;
+    a.plan_sign = attn_plan_sign(T, B, heads, kv_heads, d, max_pages, page_size);
     a.G = heads / kv_heads;
     a.Hkv = kv_heads;
     a.scale = scale;

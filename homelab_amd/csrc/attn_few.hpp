@@ -190,7 +190,7 @@ __global__ void __launch_bounds__(64 * few_waves<D>(), D == 128 && TERMS == 3 ? 
     __shared__ float mlds[few_waves<D>()][32], llds[few_waves<D>()][32];
     const int h = (int)(blockIdx.x % (uint32_t)a.Hkv), item = (int)(blockIdx.x / (uint32_t)a.Hkv);
     const AttnItem it = reinterpret_cast<const AttnItem*>(a.plan + ATTN_PLAN_HEAD + max_items * ATTN_ITEM_WORDS)[item];
-    if (item >= a.plan[ATTN_PLAN_FEW]) return;
+    if (a.plan[ATTN_PLAN_SIGN] != a.plan_sign || item >= a.plan[ATTN_PLAN_FEW]) return;
     if constexpr (attn_few_rows(D) > 16)
         if (it.rows > 16) return few_rows<D, TERMS, 32>(a, it, h, lds, mlds, llds);
     few_rows<D, TERMS, 16>(a, it, h, lds, mlds, llds);

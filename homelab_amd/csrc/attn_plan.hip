@@ -12,7 +12,7 @@ struct PlanArgs {
     const int32_t* cu_q;
     const int32_t* kv_lens;  // null: prompts, whose keys are their own tokens
     const int32_t* table;
-    int max_pages, n_pages, page_size, B, T, G, Hkv, few_rows, split_blocks;
+    int max_pages, n_pages, page_size, B, T, G, Hkv, few_rows, split_blocks, sign;
     int64_t max_items, max_few, max_merge_rows, max_part_rows;
     int32_t* positions;
     int64_t* slots;
@@ -247,8 +247,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) attn_plan_kernel(PlanArgs a) {
     }
     __syncthreads();
     if (tid == 0) {
+        a.plan[ATTN_PLAN_SIGN] = a.sign;
         a.plan[ATTN_PLAN_ITEMS] = (int)min((int64_t)items[0], a.max_items);
         a.plan[ATTN_PLAN_FEW] = (int)min((int64_t)items[1], a.max_few);
+        a.plan[ATTN_PLAN_SPLIT] = (int)min((int64_t)ks[0] * ATTN_KEYS, (int64_t)INT32_MAX);
         a.plan[ATTN_PLAN_MERGES] = (int)min((int64_t)n_merges, a.max_merge_rows);
     }
 }
@@ -292,6 +294,7 @@ extern "C" int oom_attn_plan(const int32_t* cu_q, const int32_t* kv_lens, const 
     a.Hkv = kv_heads;
     a.few_rows = attn_few_rows(d);
     a.split_blocks = attn_split_blocks(d);
+    a.sign = attn_plan_sign(T, B, heads, kv_heads, d, page_table ? max_pages : 0, page_table ? page_size : 0);
     a.max_items = p.items;
     a.max_few = p.few_items;
     a.max_merge_rows = p.merge_rows;

@@ -51,6 +51,7 @@ extern "C" int oom_attn_prompt(const void* q, int q_dtype, int64_t q_stride, con
     a.k_stride = k_stride;
     a.v_stride = v_stride;
     a.plan = plan;
+    a.plan_sign = attn_plan_sign(T, B, heads, kv_heads, d, 0, 0);
     a.G = heads / kv_heads;
     a.Hkv = kv_heads;
     a.scale = scale;

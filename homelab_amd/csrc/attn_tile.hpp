@@ -60,6 +60,7 @@ struct TileArgs {
     const int32_t* table;        // paged: [B, max_pages]
     int max_pages, n_pages, page_size;
     const int32_t* plan;
+    int plan_sign;
     int G, Hkv;
     float scale;
     float* part_ml;   // [Hkv][part rows][2]: maximum score and sum
@@ -131,8 +132,8 @@ __device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
 
 // Loads of one 64-key tile: wave w of NW takes 64 / NW rows of K and of V, which lie in one page.
 // Over pages, lane i holds the place of the wave's rows of tile i (modulo 64): looked up a tile at a
-// time, each tile waited for its page index before its loads could go out (100 tokens over 1300
-// keys 20.6 us, so 14.9).
+// time, each tile waited for its page index before its loads could go out (512 tokens over 16 Ki
+// keys 312 us, so 284).
 template <int D, int NW, bool PAGED>
 struct TileSrc {
     typedef TileLay<D> L;
@@ -328,18 +329,19 @@ __device__ __forceinline__ void tile_scores(RowState<D, TERMS, M, KEYS>& s, cons
 #pragma unroll
     for (int st = 0; st < D / S::KD; st++) {
         const int chunk = (S::KD / 8 * st + part) ^ kx;
+        tbf16x8 ka[S::NS], kf[S::NS];
 #pragma unroll
         for (int n = 0; n < S::NS; n++) {
-            if (st == 0) s.sc[n] = typename S::acc{};
             const uint4 kv = *reinterpret_cast<const uint4*>(krow + M * n * L::ROWB + 16 * chunk);
-            const tbf16x8 ka = __builtin_bit_cast(tbf16x8, kv);
-            if constexpr (TERMS > 1) {
-                const tbf16x8 kf = BAD_K ? t_finite8(ka) : ka;
-#pragma unroll
-                for (int t = TERMS - 1; t > 0; t--) s.sc[n] = Mx<M>::mul(kf, s.q[t][st], s.sc[n]);
-            }
-            s.sc[n] = Mx<M>::mul(ka, s.q[0][st], s.sc[n]);
+            ka[n] = __builtin_bit_cast(tbf16x8, kv);
+            if constexpr (TERMS > 1) kf[n] = BAD_K ? t_finite8(ka[n]) : ka[n];
+            if (st == 0) s.sc[n] = typename S::acc{};
         }
+        // products of one sum apart from each other: the next would wait for the last one's result
+#pragma unroll
+        for (int t = TERMS - 1; t >= 0; t--)
+#pragma unroll
+            for (int n = 0; n < S::NS; n++) s.sc[n] = Mx<M>::mul(t > 0 ? kf[n] : ka[n], s.q[t][st], s.sc[n]);
     }
     if constexpr (MASKED) {
 #pragma unroll
@@ -439,15 +441,32 @@ __device__ __forceinline__ void tile_values(RowState<D, TERMS, M, KEYS>& s, cons
             }
             pb[t] = __builtin_bit_cast(tbf16x8, make_uint4(b[0], b[1], b[2], b[3]));
         }
+        constexpr int DB = TERMS == 1 ? 1 : D / M < 4 ? D / M : 4;  // results whose products alternate
 #pragma unroll
-        for (int d = 0; d < D / M; d++) {
-            const uint8_t* va = vrow + S::KD * w * L::ROWB + 16 * ((M / 8 * d + vc) ^ vx);
-            const ts16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)va);
-            const ts16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(va + 256 / M * L::ROWB));
-            const uint2 w0 = __builtin_bit_cast(uint2, v0), w1 = __builtin_bit_cast(uint2, v1);
-            const tbf16x8 vv = __builtin_bit_cast(tbf16x8, make_uint4(w0.x, w0.y, w1.x, w1.y));
+        for (int d0 = 0; d0 < D / M; d0 += DB) {
+            tbf16x8 vv[DB];
 #pragma unroll
-            for (int t = TERMS - 1; t >= 0; t--) s.o[d] = Mx<M>::mul(vv, pb[t], s.o[d]);
+            for (int i = 0; i < DB; i++) {
+                const uint8_t* va = vrow + S::KD * w * L::ROWB + 16 * ((M / 8 * (d0 + i) + vc) ^ vx);
+                const ts16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)va);
+                const ts16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(va + 256 / M * L::ROWB));
+                const uint2 w0 = __builtin_bit_cast(uint2, v0), w1 = __builtin_bit_cast(uint2, v1);
+                vv[i] = __builtin_bit_cast(tbf16x8, make_uint4(w0.x, w0.y, w1.x, w1.y));
+            }
+#pragma unroll
+            for (int t = TERMS - 1; t >= 0; t--)
+#pragma unroll
+                for (int i = 0; i < DB; i++) s.o[d0 + i] = Mx<M>::mul(vv[i], pb[t], s.o[d0 + i]);
+        }
+    }
+    if constexpr (TERMS > 1) {
+        // V's operands of the next results are read before the present ones' products
+        constexpr int MFMA = 0x008, LDSR = 0x100, DB = D / M < 4 ? D / M : 4;
+        __builtin_amdgcn_sched_group_barrier(LDSR, 2 * DB, 0);
+#pragma unroll
+        for (int i = 0; i < KEYS / S::KD * (D / M) / DB; i++) {
+            __builtin_amdgcn_sched_group_barrier(LDSR, 2 * DB, 0);
+            __builtin_amdgcn_sched_group_barrier(MFMA, TERMS * DB, 0);
         }
     }
 }
@@ -553,10 +572,22 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_tile_kernel(TileArgs a) {
     const int h = (int)(blockIdx.x % (uint32_t)a.Hkv), block = (int)(blockIdx.x / (uint32_t)a.Hkv);
     const int item = block / PARTS, row_b = block % PARTS * ROWS;  // the block's first row of the tile
     AttnItem it = reinterpret_cast<const AttnItem*>(a.plan + ATTN_PLAN_HEAD)[item];
-    if (item >= a.plan[ATTN_PLAN_ITEMS] || row_b >= it.rows) return;
+    if (a.plan[ATTN_PLAN_SIGN] != a.plan_sign || item >= a.plan[ATTN_PLAN_ITEMS] || row_b >= it.rows) return;
     const int wrow = row_b + M * wave;
     const bool has = wrow < it.rows;  // uniform
     const float c = a.scale * 1.44269504088896340736f;
+    // Half tiles are twice the blocks that the plan split the keys for: a block takes two splits of its
+    // tile (an even one and the next), so that they still run at once, and leaves the second's
+    // partial empty (200 fp32 tokens over 2500 keys beside 15 single ones: 56.8 us, so 53.7).
+    int empty = 0;  // rows from its partial to the second's, if there is one
+    if constexpr (PARTS > 1 && PAGED) {
+        const int split = a.plan[ATTN_PLAN_SPLIT], keys = it.off + 1 + (int)((uint32_t)(it.row0 + it.rows - 1) / (uint32_t)a.G);
+        if (it.part >= 0 && it.k0 / split % 2 != 0) return;
+        if (it.part >= 0 && it.k1 < keys) {
+            it.k1 = min(keys, it.k1 + split);
+            empty = it.rows;
+        }
+    }
     // no row of the block sees keys past its last row's position
     if constexpr (PARTS > 1)
         it.k1 = min(it.k1, it.off + 1 + (int)((uint32_t)(it.row0 + min(row_b + ROWS, it.rows) - 1) / (uint32_t)a.G));
@@ -629,6 +660,9 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_tile_kernel(TileArgs a) {
     __syncthreads();  // every wave is done with the tiles
     static_assert(4 * L::BYTES >= NW * M * D * 4, "the rows fit the tiles' places");
     if (has) rows_store(s, a, it, h, wrow, lane, tiles + wave * (M * D * 4));
+    if (empty > 0 && lane < M && s.live)
+        *reinterpret_cast<float2*>(a.part_ml + 2 * ((int64_t)h * a.part_rows + it.part + empty + wrow + lane)) =
+            make_float2(-INFINITY, 0.0f);
 }
 
 // Rows a wave: 32 up to d 128 in one term; 16 for three terms and for d 256, whose Q and O of 32 rows

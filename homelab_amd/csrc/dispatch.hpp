@@ -316,7 +316,21 @@ constexpr int attn_split_blocks(int d) { return d == 256 ? 256 : 512; }
 // and the rows to merge.
 constexpr int ATTN_PLAN_HEAD = 16;
 constexpr int ATTN_ITEM_WORDS = 8, ATTN_MERGE_WORDS = 4;
-constexpr int ATTN_PLAN_ITEMS = 0, ATTN_PLAN_FEW = 1, ATTN_PLAN_MERGES = 2;  // head words: how many of each
+constexpr int ATTN_PLAN_ITEMS = 0, ATTN_PLAN_FEW = 1, ATTN_PLAN_MERGES = 2;  // head words: how many of each,
+constexpr int ATTN_PLAN_SPLIT = 3;                                          // the items' keys a split,
+constexpr int ATTN_PLAN_SIGN = 4;                                           // and what it was made for
+
+// What a plan is made for, in a word: the attention kernels do nothing on a plan of other sizes (or on
+// words that no plan was written to), whose items would point anywhere.
+inline int32_t attn_plan_sign(int64_t T, int64_t B, int64_t heads, int64_t kv_heads, int64_t d, int64_t max_pages,
+                              int64_t page_size) {
+    uint64_t h = 0x9e3779b97f4a7c15ull;
+    for (int64_t v : {T, B, heads, kv_heads, d, max_pages, page_size}) {
+        h = (h ^ (uint64_t)v) * 0xff51afd7ed558ccdull;
+        h ^= h >> 33;
+    }
+    return (int32_t)h;
+}
 
 // The plan's bounds, from sizes that the host knows. Tiles of sequence b: ceil(n_b G / 128), so at
 // most T G / 128 + B in all. With W key tiles over them and splits of ks = ceil(W Hkv /

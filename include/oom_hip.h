@@ -450,7 +450,9 @@ int oom_rope_append_paged(const void* q, int64_t q_stride, const void* k, int64_
 
 /* The plan of one step's batch of B sequences (at most 4096), made on the device from device
  * lengths and used by the attention calls of every layer with the same T, B, heads, kv_heads
- * and d: `plan` holds oom_attn_plan_size() i32 words, 16-byte aligned.
+ * and d (and max_pages, page_size): `plan` holds oom_attn_plan_size() i32 words, 16-byte aligned. A
+ * plan made for other sizes, or never made, is told by a word in it: the call writes nothing.
+ * The lengths that it was made from must be those of the call: new lengths, a new plan.
  *   cu_q i32 [B + 1], rising from 0 or more to at most T;
  *   kv_lens i32 [B]: keys in the cache after this step's tokens are written (new token i of n is
  *   at position kv_len - n + i; a negative position sees nothing), page_table i32 [B, max_pages];
@@ -465,7 +467,7 @@ int oom_attn_plan(const int32_t* cu_q, const int32_t* kv_lens, const int32_t* pa
 /* Causal attention of packed prompts: out[t, h, :] = sum_j softmax_j(q[t, h] . k[j, g] * scale)
  * v[j, g] over the tokens j of t's sequence up to t, g = h / (heads / kv_heads). q [T, heads, d] in
  * q_dtype; k and v bf16 [T, kv_heads, d]; out [T, heads, d] in out_dtype. d 64, 128 or 256; any
- * number of query heads a KV head; scale positive. plan: oom_attn_plan's with null kv_lens.
+ * number of query heads a KV head; scale positive; out overlaps no input. plan: oom_attn_plan's with null kv_lens.
  * Keys that a token does not see have no part in its row, whatever they hold. fp32 on either
  * side: fp32 products, sums and exponentials (three exact bf16 terms on the matrix cores);
  * bf16 on both: the weights p enter the second product rounded to bf16, sums in fp32.
@@ -476,8 +478,8 @@ int oom_attn_prompt(const void* q, int q_dtype, int64_t q_stride, const uint16_t
                     int d, float scale, void* out, int out_dtype, int64_t out_stride, void* stream);
 /* Attention of a step's new tokens, one or many a sequence, over the paged cache that already
  * holds their rows: the token at position p sees the keys 0 .. p of its sequence; a token that
- * sees none gets zeros. max_q bounds the new tokens of any sequence (1: a decode step). plan:
- * oom_attn_plan's with kv_lens and page_table. A page index outside [0, n_pages) reads zeros.
+ * sees none gets zeros. max_q bounds the new tokens of any sequence (1: a decode step; a longer one's
+ * rows may be left unwritten). plan: oom_attn_plan's with kv_lens and page_table. A page index outside [0, n_pages) reads zeros.
  * Types, products and heads as oom_attn_prompt, page_size a multiple of 16. */
 size_t oom_attn_chunk_paged_workspace_size(int T, int B, int heads, int kv_heads, int d);
 int oom_attn_chunk_paged(const void* q, int q_dtype, int64_t q_stride, const uint16_t* k_pages,

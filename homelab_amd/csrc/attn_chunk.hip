@@ -75,19 +75,22 @@ __global__ void __launch_bounds__(256) attn_rows_merge_kernel(TileArgs a, const 
     }
 }
 
-// The kernels that a batch may need: sequences of more than attn_few_rows() rows there are only where max_q new
-// tokens have them, few-row ones only beside others, or where max_q leaves no others.
+// The kernels that a batch may need: sequences of more than attn_few_rows() rows there are only where
+// max_q new tokens have them, few-row ones only beside others, or where max_q leaves no others.
+template <int D, int TERMS>
+static void launch_rows(const TileArgs& a, const AttnPlanDims& p, int B, int max_q, hipStream_t st) {
+    const bool tiles = (int64_t)max_q * a.G > attn_few_rows(D), few = !tiles || B > 1;
+    if constexpr (D <= 128)
+        if (tiles && few) return launch_mixed<D, TERMS>(a, p, st);
+    if (tiles) launch_tiles<D, TERMS, true>(a, p.items, st);
+    if (few) launch_few<D, TERMS>(a, p, st);
+}
+
 template <int D>
 static int launch_chunk(const TileArgs& a, const AttnPlanDims& p, int B, int max_q, bool exact, hipStream_t st) {
-    const int64_t most = (int64_t)max_q * a.G;
-    if (most > attn_few_rows(D)) {
-        launch_tiles<D, true>(a, p.items, exact, st);
-        if (int rc = launched("oom_attn_chunk_paged")) return rc;
-    }
-    if (most <= attn_few_rows(D) || B > 1) {
-        launch_few<D>(a, p, exact, st);
-        if (int rc = launched("oom_attn_chunk_paged")) return rc;
-    }
+    if (exact) launch_rows<D, 3>(a, p, B, max_q, st);
+    else launch_rows<D, 1>(a, p, B, max_q, st);
+    if (int rc = launched("oom_attn_chunk_paged")) return rc;
     const int4* rows = reinterpret_cast<const int4*>(a.plan + ATTN_PLAN_HEAD + (p.items + p.few_items) * ATTN_ITEM_WORDS);
     const dim3 grid((uint32_t)std::min<int64_t>(2048, cdiv(p.merge_rows * a.Hkv, 4)));
     hipLaunchKernelGGL((attn_rows_merge_kernel<D>), grid, dim3(256), 0, st, a, rows);
@@ -127,7 +130,7 @@ extern "C" int oom_attn_chunk_paged(const void* q, int q_dtype, int64_t q_stride
     OOM_REQUIRE(aligned(q, 16) && aligned(k_pages, 16) && aligned(v_pages, 16) && aligned(out, 16) && aligned(plan, 16),
                 "oom_attn_chunk_paged: q, k_pages, v_pages, out and plan must be 16-byte aligned");
     const AttnPlanDims p = attn_plan_dims(T, B, heads, kv_heads, d);
-    OOM_REQUIRE(p.items * kv_heads < (1ll << 30), "oom_attn_chunk_paged: too many tiles of rows");
+    OOM_REQUIRE((p.items + p.few_items) * kv_heads < (1ll << 30), "oom_attn_chunk_paged: too many tiles of rows");
     if (!ws || ws_bytes < oom_attn_chunk_paged_workspace_size(T, B, heads, kv_heads, d))
         return fail(OOM_ERR_WORKSPACE,
                     "oom_attn_chunk_paged: workspace smaller than oom_attn_chunk_paged_workspace_size()");

@@ -183,12 +183,14 @@ __device__ __forceinline__ void few_rows(const TileArgs& a, const AttnItem& it, 
     }
 }
 
+template <int D>
+constexpr int few_lds() { return few_waves<D>() * 2 * FK * TileLay<D>::ROWB; }
+
 // Block i takes few-row item i / Hkv for KV head i % Hkv, with as many rows a wave as it needs.
 template <int D, int TERMS>
-__global__ void __launch_bounds__(64 * few_waves<D>(), D == 128 && TERMS == 3 ? 1 : 2) attn_few_kernel(TileArgs a, int64_t max_items) {
-    __shared__ __align__(16) uint8_t lds[few_waves<D>() * 2 * FK * TileLay<D>::ROWB];
-    __shared__ float mlds[few_waves<D>()][32], llds[few_waves<D>()][32];
-    const int h = (int)(blockIdx.x % (uint32_t)a.Hkv), item = (int)(blockIdx.x / (uint32_t)a.Hkv);
+__device__ __forceinline__ void few_block(const TileArgs& a, uint32_t index, int64_t max_items, uint8_t* lds,
+                                          float (&mlds)[few_waves<D>()][32], float (&llds)[few_waves<D>()][32]) {
+    const int h = (int)(index % (uint32_t)a.Hkv), item = (int)(index / (uint32_t)a.Hkv);
     const AttnItem it = reinterpret_cast<const AttnItem*>(a.plan + ATTN_PLAN_HEAD + max_items * ATTN_ITEM_WORDS)[item];
     if (a.plan[ATTN_PLAN_SIGN] != a.plan_sign || item >= a.plan[ATTN_PLAN_FEW]) return;
     if constexpr (attn_few_rows(D) > 16)
@@ -196,11 +198,39 @@ __global__ void __launch_bounds__(64 * few_waves<D>(), D == 128 && TERMS == 3 ? 
     few_rows<D, TERMS, 16>(a, it, h, lds, mlds, llds);
 }
 
-template <int D>
-void launch_few(const TileArgs& a, const AttnPlanDims& p, bool exact, hipStream_t st) {
-    const dim3 grid((uint32_t)(p.few_items * a.Hkv)), block(64 * few_waves<D>());
-    if (exact) hipLaunchKernelGGL((attn_few_kernel<D, 3>), grid, block, 0, st, a, p.items);
-    else hipLaunchKernelGGL((attn_few_kernel<D, 1>), grid, block, 0, st, a, p.items);
+template <int D, int TERMS>
+__global__ void __launch_bounds__(64 * few_waves<D>(), D == 128 && TERMS == 3 ? 1 : 2)
+    attn_few_kernel(TileArgs a, int64_t max_items) {
+    __shared__ __align__(16) uint8_t lds[few_lds<D>()];
+    __shared__ float mlds[few_waves<D>()][32], llds[few_waves<D>()][32];
+    few_block<D, TERMS>(a, blockIdx.x, max_items, lds, mlds, llds);
+}
+
+template <int D, int TERMS>
+void launch_few(const TileArgs& a, const AttnPlanDims& p, hipStream_t st) {
+    hipLaunchKernelGGL((attn_few_kernel<D, TERMS>), dim3((uint32_t)(p.few_items * a.Hkv)), dim3(64 * few_waves<D>()), 0, st, a,
+                       p.items);
+}
+
+// Both kinds of a mixed batch in one launch (d up to 128: the same block and LDS): the tiles first,
+// which are the longer, then the few-row sequences, which fill the CUs that the last tiles leave
+// idle.
+template <int D, int TERMS>
+__global__ void __launch_bounds__(256, 2) attn_mixed_kernel(TileArgs a, int64_t max_items, uint32_t tile_blocks) {
+    typedef TileShape<D, TERMS> S;
+    static_assert(S::NW == 4 && few_waves<D>() == 4, "one block size");
+    __shared__ __align__(16) uint8_t lds[tile_lds<D>() > few_lds<D>() ? tile_lds<D>() : few_lds<D>()];
+    __shared__ float mlds[4][32], llds[4][32];
+    __shared__ uint32_t bad_lds[4];
+    if (blockIdx.x < tile_blocks) tile_block<D, TERMS, S::M, 4, true>(a, blockIdx.x, lds, bad_lds);
+    else few_block<D, TERMS>(a, blockIdx.x - tile_blocks, max_items, lds, mlds, llds);
+}
+
+template <int D, int TERMS>
+void launch_mixed(const TileArgs& a, const AttnPlanDims& p, hipStream_t st) {
+    const uint32_t tiles = (uint32_t)(p.items * a.Hkv * TileShape<D, TERMS>::PARTS);
+    hipLaunchKernelGGL((attn_mixed_kernel<D, TERMS>), dim3(tiles + (uint32_t)(p.few_items * a.Hkv)), dim3(256), 0, st, a, p.items,
+                       tiles);
 }
 
 }  // namespace oom

@@ -8,7 +8,8 @@ namespace oom {
 
 template <int D>
 static int launch_prompt(const TileArgs& a, int64_t items, bool exact, hipStream_t st) {
-    launch_tiles<D, false>(a, items, exact, st);
+    if (exact) launch_tiles<D, 3, false>(a, items, st);
+    else launch_tiles<D, 1, false>(a, items, st);
     return launched("oom_attn_prompt");
 }
 

@@ -560,16 +560,17 @@ __device__ __forceinline__ void rows_store(RowState<D, TERMS, M>& s, const TileA
 // K and V tiles go through LDS in two stages, one barrier a tile: past it, every wave has done
 // with the stage that the next tile's loads now fill, and those have a whole tile to arrive.
 // Two blocks a CU (d up to 128) or two waves a SIMD take turns on the matrix cores and the
-// vector units.
+// vector units. bad_lds: per stage, K and V hold infinities or NaN.
+template <int D>
+constexpr int tile_lds() { return 4 * TileLay<D>::BYTES; }  // stage 0: K, V; stage 1: K, V
+
 template <int D, int TERMS, int M, int NW, bool PAGED>
-__global__ void __launch_bounds__(64 * NW, 2) attn_tile_kernel(TileArgs a) {
+__device__ __forceinline__ void tile_block(const TileArgs& a, uint32_t index, uint8_t* tiles, uint32_t (&bad_lds)[4]) {
     typedef TileLay<D> L;
     constexpr int ROWS = NW * M, PARTS = ATTN_ROWS / ROWS;
-    __shared__ __align__(16) uint8_t tiles[4 * L::BYTES];  // stage 0: K, V; stage 1: K, V
-    __shared__ uint32_t bad_lds[4];                        // per stage: K, V hold infinities or NaN
     const int lane = threadIdx.x & 63;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int h = (int)(blockIdx.x % (uint32_t)a.Hkv), block = (int)(blockIdx.x / (uint32_t)a.Hkv);
+    const int h = (int)(index % (uint32_t)a.Hkv), block = (int)(index / (uint32_t)a.Hkv);
     const int item = block / PARTS, row_b = block % PARTS * ROWS;  // the block's first row of the tile
     AttnItem it = reinterpret_cast<const AttnItem*>(a.plan + ATTN_PLAN_HEAD)[item];
     if (a.plan[ATTN_PLAN_SIGN] != a.plan_sign || item >= a.plan[ATTN_PLAN_ITEMS] || row_b >= it.rows) return;
@@ -669,14 +670,29 @@ __global__ void __launch_bounds__(64 * NW, 2) attn_tile_kernel(TileArgs a) {
 // leave no registers for a second wave on the SIMD. Waves a block: a tile's rows, but half of
 // them for three terms up to d 128, so that two blocks fit a CU and do not wait at the same
 // barriers (LDS holds one block at d 256).
-template <int D, bool PAGED>
-void launch_tiles(const TileArgs& a, int64_t items, bool exact, hipStream_t st) {
-    constexpr int M1 = D <= 128 ? 32 : 16, NW1 = ATTN_ROWS / M1, NW3 = D <= 128 ? 4 : 8;
-    const int64_t n = items * a.Hkv;
-    if (exact)
-        hipLaunchKernelGGL((attn_tile_kernel<D, 3, 16, NW3, PAGED>), dim3((uint32_t)(n * (8 / NW3))), dim3(64 * NW3), 0, st, a);
-    else
-        hipLaunchKernelGGL((attn_tile_kernel<D, 1, M1, NW1, PAGED>), dim3((uint32_t)n), dim3(64 * NW1), 0, st, a);
+template <int D, int TERMS>
+struct TileShape {
+    static constexpr int M = D <= 128 && TERMS == 1 ? 32 : 16;
+    static constexpr int NW = D <= 128 ? 4 : 8;  // 64 NW threads: tile_threads()
+    static constexpr int PARTS = ATTN_ROWS / (M * NW);  // blocks a tile
+};
+
+template <int D>
+constexpr int tile_threads() { return D <= 128 ? 256 : 512; }
+
+template <int D, int TERMS, bool PAGED>
+__global__ void __launch_bounds__(tile_threads<D>(), 2) attn_tile_kernel(TileArgs a) {
+    typedef TileShape<D, TERMS> S;
+    __shared__ __align__(16) uint8_t tiles[tile_lds<D>()];
+    __shared__ uint32_t bad_lds[4];
+    tile_block<D, TERMS, S::M, S::NW, PAGED>(a, blockIdx.x, tiles, bad_lds);
+}
+
+template <int D, int TERMS, bool PAGED>
+void launch_tiles(const TileArgs& a, int64_t items, hipStream_t st) {
+    typedef TileShape<D, TERMS> S;
+    hipLaunchKernelGGL((attn_tile_kernel<D, TERMS, PAGED>), dim3((uint32_t)(items * a.Hkv * S::PARTS)), dim3(64 * S::NW), 0,
+                       st, a);
 }
 
 }  // namespace oom

@@ -27,6 +27,13 @@ __device__ __forceinline__ void f_wait_loads() {
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
+// This wave's LDS reads are done: what they read may be written over by loads.
+__device__ __forceinline__ void f_wait_reads() {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0); vmcnt and expcnt left at their maxima
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
 template <int D, int TERMS, int M>
 __device__ __forceinline__ void few_rows(const TileArgs& a, const AttnItem& it, int h, uint8_t* lds,
                                          float (&mlds)[few_waves<D>()][32], float (&llds)[few_waves<D>()][32]) {
@@ -109,7 +116,10 @@ __device__ __forceinline__ void few_rows(const TileArgs& a, const AttnItem& it, 
             find_places(t + 1);
             t_wait_loads();
         }
-        if (more) load(t + 1, kb, ko, k_at);
+        if (more) {
+            f_wait_reads();
+            load(t + 1, kb, ko, k_at);
+        }
         const float mb = tile_maximum(s, c);
         if (more) f_wait_loads<LOADS>();
         else f_wait_loads<0>();
@@ -124,7 +134,10 @@ __device__ __forceinline__ void few_rows(const TileArgs& a, const AttnItem& it, 
             wave_lds_order();
         }
         tile_values(s, vt, c, mb, lane);
-        if (more) load(t + 1, vb, vo, v_at);
+        if (more) {
+            f_wait_reads();
+            load(t + 1, vb, vo, v_at);
+        }
     };
     for (int t = 0; t < n; t++) {
         if (key0(t) + FK - 1 > lo || key0(t) + FK > it.k1) step(t, std::true_type{});

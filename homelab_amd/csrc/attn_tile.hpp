@@ -32,7 +32,6 @@ typedef float tf32x16 __attribute__((ext_vector_type(16)));
 typedef short ts16x4 __attribute__((ext_vector_type(4)));
 typedef __attribute__((address_space(3))) ts16x4* tr_ptr_t;
 typedef __attribute__((address_space(3))) void* t_lds_t;
-typedef const __attribute__((address_space(1))) void* t_glb_t;
 
 constexpr float T_GROW = 8.0f;  // growth of a row's maximum (log2) that rescales O
 

@@ -266,21 +266,21 @@ extern "C" int oom_rope_table(const OomRope* rope, uint64_t* turns, size_t n, fl
 namespace oom {
 
 static int rope_checks(const char* what, const RopeArgs& a, int layout, int x_dtype, int out_dtype) {
-    const std::string w = what;
-    OOM_REQUIRE(a.d >= 8 && a.d % 8 == 0 && a.d <= 1024, w + ": head_dim must be a multiple of 8 up to 1024");
-    OOM_REQUIRE(a.rot >= 2 && a.rot % 2 == 0 && a.rot <= a.d, w + ": rot_dim must be even, at most head_dim");
-    OOM_REQUIRE(layout == OOM_ROPE_HALF || layout == OOM_ROPE_INTERLEAVED, w + ": layout");
-    OOM_REQUIRE(x_dtype == OOM_F32 || x_dtype == OOM_BF16, w + ": x_dtype");
-    OOM_REQUIRE(out_dtype == OOM_F32 || out_dtype == OOM_BF16, w + ": out_dtype");
-    OOM_REQUIRE(a.T >= 0 && a.H >= 1 && a.H <= 4096, w + ": T must be >= 0, heads 1 to 4096");
-    OOM_REQUIRE(std::isfinite(a.magnitude), w + ": magnitude must be finite");
+    const auto w = [what](const char* msg) { return std::string(what) + msg; };
+    OOM_REQUIRE(a.d >= 8 && a.d % 8 == 0 && a.d <= 1024, w(": head_dim must be a multiple of 8 up to 1024"));
+    OOM_REQUIRE(a.rot >= 2 && a.rot % 2 == 0 && a.rot <= a.d, w(": rot_dim must be even, at most head_dim"));
+    OOM_REQUIRE(layout == OOM_ROPE_HALF || layout == OOM_ROPE_INTERLEAVED, w(": layout"));
+    OOM_REQUIRE(x_dtype == OOM_F32 || x_dtype == OOM_BF16, w(": x_dtype"));
+    OOM_REQUIRE(out_dtype == OOM_F32 || out_dtype == OOM_BF16, w(": out_dtype"));
+    OOM_REQUIRE(a.T >= 0 && a.H >= 1 && a.H <= 4096, w(": T must be >= 0, heads 1 to 4096"));
+    OOM_REQUIRE(std::isfinite(a.magnitude), w(": magnitude must be finite"));
     OOM_REQUIRE(a.q_stride >= (int64_t)a.H * a.d && a.out_stride >= (int64_t)a.H * a.d && a.q_stride % 8 == 0 &&
                     a.out_stride % 8 == 0,
-                w + ": strides must be multiples of 8 elements, at least a token's heads");
+                w(": strides must be multiples of 8 elements, at least a token's heads"));
     if (a.T == 0) return OOM_OK;
-    OOM_REQUIRE(a.q && a.out && a.positions && a.turns, w + ": null buffer");
+    OOM_REQUIRE(a.q && a.out && a.positions && a.turns, w(": null buffer"));
     OOM_REQUIRE(aligned(a.q, 16) && aligned(a.out, 16) && aligned(a.turns, 8),
-                w + ": buffers of heads must be 16-byte aligned");
+                w(": buffers of heads must be 16-byte aligned"));
     return OOM_OK;
 }
 

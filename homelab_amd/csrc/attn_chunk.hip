@@ -1,7 +1,5 @@
 // Attention of each sequence's new tokens over its paged cache (oom_attn_chunk_paged): attn_tile.hpp
 // over pages, then the merge of the row tiles whose keys were split.
-#include <cmath>
-
 #include "attn_few.hpp"
 
 namespace oom {
@@ -121,7 +119,7 @@ extern "C" int oom_attn_chunk_paged(const void* q, int q_dtype, int64_t q_stride
                 "oom_attn_chunk_paged: n_pages and max_pages must be >= 1, a sequence at most 128 Mi keys");
     OOM_REQUIRE(q_dtype == OOM_F32 || q_dtype == OOM_BF16, "oom_attn_chunk_paged: q_dtype");
     OOM_REQUIRE(out_dtype == OOM_F32 || out_dtype == OOM_BF16, "oom_attn_chunk_paged: out_dtype");
-    OOM_REQUIRE(scale > 0.0f && std::isfinite(scale), "oom_attn_chunk_paged: scale must be positive and finite");
+    OOM_REQUIRE(scale >= 0x1p-60f && scale <= 0x1p60f, "oom_attn_chunk_paged: scale must be from 2^-60 to 2^60");
     OOM_REQUIRE(q_stride >= (int64_t)heads * d && out_stride >= (int64_t)heads * d && q_stride % 8 == 0 &&
                     out_stride % 8 == 0,
                 "oom_attn_chunk_paged: strides must be multiples of 8 elements, at least a token's heads");

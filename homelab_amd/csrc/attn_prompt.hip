@@ -1,7 +1,5 @@
 // Causal attention of packed prompts (oom_attn_prompt): attn_tile.hpp over the K and V rows of the
 // prompts' own tokens.
-#include <cmath>
-
 #include "attn_tile.hpp"
 
 namespace oom {
@@ -27,7 +25,7 @@ extern "C" int oom_attn_prompt(const void* q, int q_dtype, int64_t q_stride, con
                 "oom_attn_prompt: at most 4096 sequences, and fewer than 2^31 rows of heads");
     OOM_REQUIRE(q_dtype == OOM_F32 || q_dtype == OOM_BF16, "oom_attn_prompt: q_dtype");
     OOM_REQUIRE(out_dtype == OOM_F32 || out_dtype == OOM_BF16, "oom_attn_prompt: out_dtype");
-    OOM_REQUIRE(scale > 0.0f && std::isfinite(scale), "oom_attn_prompt: scale must be positive and finite");
+    OOM_REQUIRE(scale >= 0x1p-60f && scale <= 0x1p60f, "oom_attn_prompt: scale must be from 2^-60 to 2^60");
     OOM_REQUIRE(q_stride >= (int64_t)heads * d && out_stride >= (int64_t)heads * d &&
                     k_stride >= (int64_t)kv_heads * d && v_stride >= (int64_t)kv_heads * d,
                 "oom_attn_prompt: strides smaller than a token's heads");

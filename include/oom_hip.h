@@ -467,7 +467,8 @@ int oom_attn_plan(const int32_t* cu_q, const int32_t* kv_lens, const int32_t* pa
 /* Causal attention of packed prompts: out[t, h, :] = sum_j softmax_j(q[t, h] . k[j, g] * scale)
  * v[j, g] over the tokens j of t's sequence up to t, g = h / (heads / kv_heads). q [T, heads, d] in
  * q_dtype; k and v bf16 [T, kv_heads, d]; out [T, heads, d] in out_dtype. d 64, 128 or 256; any
- * number of query heads a KV head; scale positive; out overlaps no input. plan: oom_attn_plan's with null kv_lens.
+ * number of query heads a KV head; scale from 2^-60 to 2^60; out overlaps no input. plan:
+ * oom_attn_plan's with null kv_lens.
  * Keys that a token does not see have no part in its row, whatever they hold. fp32 on either
  * side: fp32 products, sums and exponentials (three exact bf16 terms on the matrix cores);
  * bf16 on both: the weights p enter the second product rounded to bf16, sums in fp32.
@@ -479,7 +480,8 @@ int oom_attn_prompt(const void* q, int q_dtype, int64_t q_stride, const uint16_t
 /* Attention of a step's new tokens, one or many a sequence, over the paged cache that already
  * holds their rows: the token at position p sees the keys 0 .. p of its sequence; a token that
  * sees none gets zeros. max_q bounds the new tokens of any sequence (1: a decode step; a longer one's
- * rows may be left unwritten). plan: oom_attn_plan's with kv_lens and page_table. A page index outside [0, n_pages) reads zeros.
+ * rows may be left unwritten). plan: oom_attn_plan's with kv_lens and page_table. A page index
+ * outside [0, n_pages) reads zeros.
  * Types, products and heads as oom_attn_prompt, page_size a multiple of 16. */
 size_t oom_attn_chunk_paged_workspace_size(int T, int B, int heads, int kv_heads, int d);
 int oom_attn_chunk_paged(const void* q, int q_dtype, int64_t q_stride, const uint16_t* k_pages,

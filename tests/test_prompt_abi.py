@@ -133,7 +133,7 @@ def prompt_args(**kw):
 @pytest.mark.parametrize("kw,text", [
     (dict(d=80), "head_dim"), (dict(heads=7), "multiple of kv_heads"), (dict(B=4097), "4096 sequences"),
     (dict(qdt=2), "q_dtype"), (dict(odt=2), "out_dtype"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"),
-    (dict(scale=math.inf), "scale"), (dict(scale=math.nan), "scale"), (dict(qs=1016), "strides"), (dict(ks=248), "strides"),
+    (dict(scale=math.inf), "scale"), (dict(scale=math.nan), "scale"), (dict(scale=1e-30), "scale"), (dict(scale=1e30), "scale"), (dict(qs=1016), "strides"), (dict(ks=248), "strides"),
     (dict(vs=260), "strides"), (dict(os=1030), "strides"), (dict(ks=1 << 25), "strides"), (dict(q=NULL), "null"),
     (dict(k=NULL), "null"), (dict(plan=NULL), "null"), (dict(out=NULL), "null"), (dict(v=ctypes.c_void_p(4104)), "16-byte"),
 ])

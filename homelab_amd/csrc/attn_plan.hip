@@ -13,7 +13,7 @@ struct PlanArgs {
     const int32_t* kv_lens;  // null: prompts, whose keys are their own tokens
     const int32_t* table;
     int max_pages, n_pages, page_size, B, T, G, Hkv, few_rows, split_blocks, sign;
-    int64_t max_items, max_few, max_merge_rows, max_part_rows;
+    int64_t max_items, max_few, max_merge_rows;
     int32_t* positions;
     int64_t* slots;
     int32_t* plan;
@@ -235,10 +235,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) attn_plan_kernel(PlanArgs a) {
             }
             part = __shfl(part, 0);
             m = __shfl(m, 0);
-            if (part + (int64_t)n * s.rows > a.max_part_rows || m + (int64_t)s.rows > a.max_merge_rows) continue;
             // a row to merge: its token, its head of the group (bit 30: it sees no key), its first
-            // partial, and how many there are, s.rows apart
-            for (int r = lane; r < s.rows; r += 64) {
+            // partial, and how many there are, s.rows apart. (The partials fit whatever cu_q holds, since
+            // their bound follows from the split; rows to merge are more than there is room for
+            // only where sequences overlap.)
+            for (int r = lane; r < s.rows && m + (int64_t)r < a.max_merge_rows; r += 64) {
                 const int tok = (s.row0 + r) / a.G, g = s.row0 + r - tok * a.G;
                 merges[m + r] = make_int4(s.q0 + tok, g | (s.off + tok < 0 ? 1 << 30 : 0), part + r, n | s.rows << 16);
             }
@@ -298,7 +299,6 @@ extern "C" int oom_attn_plan(const int32_t* cu_q, const int32_t* kv_lens, const 
     a.max_items = p.items;
     a.max_few = p.few_items;
     a.max_merge_rows = p.merge_rows;
-    a.max_part_rows = p.part_rows;
     a.positions = positions;
     a.slots = slots;
     a.plan = plan;

@@ -453,7 +453,8 @@ int oom_rope_append_paged(const void* q, int64_t q_stride, const void* k, int64_
  * and d (and max_pages, page_size): `plan` holds oom_attn_plan_size() i32 words, 16-byte aligned. A
  * plan made for other sizes, or never made, is told by a word in it: the call writes nothing.
  * The lengths that it was made from must be those of the call: new lengths, a new plan.
- *   cu_q i32 [B + 1], rising from 0 or more to at most T;
+ *   cu_q i32 [B + 1], rising from 0 or more to at most T (where it does not rise, sequences are cut
+ *   to [0, T), and the rows that more than one of them claims may hold anything);
  *   kv_lens i32 [B]: keys in the cache after this step's tokens are written (new token i of n is
  *   at position kv_len - n + i; a negative position sees nothing), page_table i32 [B, max_pages];
  *   both null for prompts (oom_attn_prompt), whose keys are their own tokens.

@@ -271,6 +271,33 @@ def test_batches_that_do_not_rise_touch_nothing_else(hip):
         assert bool((out[top:] == 3.0).all())
 
 
+@pytest.mark.parametrize("cu", [[0, 64, 0, 64], [0, 8, 0, 8, 0, 8, 0], [64, 0, 64, 8, 64, 0], [-70, 64, -1, 90]])
+def test_plans_of_overlapping_sequences_hold_nothing_unwritten(hip, cu):
+    """Sequences over the same tokens have more rows to merge than the batch has rows: the plan's counts stay
+    within what it wrote, and each entry within the batch."""
+    g = pc.gen(20)
+    T, H, Hkv, d, page, B = 64, 4, 1, 64, 16, len(cu) - 1
+    kv = [3000 + b for b in range(B)]
+    kp, vp, table = pc.paged(g, kv, Hkv, d, page)
+    q = pc.randn(g, (T, H, d), BF)
+    plan = torch.full((hip.attn_plan_size(T, B, H, Hkv, d),), -9, dtype=torch.int32, device="cuda")
+    hip.attn_plan(torch.tensor(cu, dtype=torch.int32, device="cuda"), torch.tensor(kv, dtype=torch.int32, device="cuda"), table,
+                  T, H, Hkv, d, plan, n_pages=kp.shape[0], page_size=page)
+    one, two, rows = listed(plan, T, B, H, Hkv, d)
+    size = hip.attn_chunk_paged_workspace_size(T, B, H, Hkv, d)
+    parts = size // (Hkv * (d + 2) * 4)
+    assert one or two
+    for q0, r0, r, off, k0, k1, part, b in one + two:
+        assert 0 <= b < B and r > 0 and r0 >= 0 and q0 >= 0 and q0 * H + r0 + r <= T * H
+        assert 0 <= k0 < k1 <= kv[b] and (part == -1 or 0 <= part <= parts - r)
+    for tok, head, part, n in rows:
+        assert 0 <= tok < T and 0 <= head < H and part >= 0 and part + (n >> 16) * ((n & 0xffff) - 1) < parts
+    out = torch.full((T, H, d), 3.0, dtype=BF, device="cuda")
+    ws = torch.zeros(size, dtype=torch.uint8, device="cuda")
+    hip.attn_chunk_paged(q, kp, vp, table, plan, T, 0.125, out, ws)
+    assert bool(out.isfinite().all())
+
+
 # ---- the largest offsets ---------------------------------------------------------------------
 
 

@@ -73,11 +73,11 @@ __global__ void __launch_bounds__(256) attn_rows_merge_kernel(TileArgs a, const 
     }
 }
 
-// The kernels that a batch may need: sequences of more than attn_few_rows() rows there are only where
-// max_q new tokens have them, few-row ones only beside others, or where max_q leaves no others.
+// The kernels that a batch may need. Tiles: where max_q new tokens have more rows than a few-row
+// sequence, or the batch's lone sequence is none by its kind.
 template <int D, int TERMS>
-static void launch_rows(const TileArgs& a, const AttnPlanDims& p, int B, int max_q, hipStream_t st) {
-    const bool tiles = (int64_t)max_q * a.G > attn_few_rows(D), few = !tiles || B > 1;
+static void launch_rows(const TileArgs& a, const AttnPlanDims& p, int64_t T, int B, int max_q, hipStream_t st) {
+    const bool few = attn_has_few(T, B, a.G, D), tiles = !few || (int64_t)max_q * a.G > attn_few_rows(D);
     if constexpr (D <= 128)
         if (tiles && few) return launch_mixed<D, TERMS>(a, p, st);
     if (tiles) launch_tiles<D, TERMS, true>(a, p.items, st);
@@ -85,9 +85,9 @@ static void launch_rows(const TileArgs& a, const AttnPlanDims& p, int B, int max
 }
 
 template <int D>
-static int launch_chunk(const TileArgs& a, const AttnPlanDims& p, int B, int max_q, bool exact, hipStream_t st) {
-    if (exact) launch_rows<D, 3>(a, p, B, max_q, st);
-    else launch_rows<D, 1>(a, p, B, max_q, st);
+static int launch_chunk(const TileArgs& a, const AttnPlanDims& p, int T, int B, int max_q, bool exact, hipStream_t st) {
+    if (exact) launch_rows<D, 3>(a, p, T, B, max_q, st);
+    else launch_rows<D, 1>(a, p, T, B, max_q, st);
     if (int rc = launched("oom_attn_chunk_paged")) return rc;
     const int4* rows = reinterpret_cast<const int4*>(a.plan + ATTN_PLAN_HEAD + (p.items + p.few_items) * ATTN_ITEM_WORDS);
     const dim3 grid((uint32_t)std::min<int64_t>(2048, cdiv(p.merge_rows * a.Hkv, 4)));
@@ -156,7 +156,7 @@ extern "C" int oom_attn_chunk_paged(const void* q, int q_dtype, int64_t q_stride
     a.part_ml = a.part_acc + p.part_rows * kv_heads * d;
     const bool exact = q_dtype == OOM_F32 || out_dtype == OOM_F32;
     hipStream_t st = as_stream(stream);
-    if (d == 64) return launch_chunk<64>(a, p, B, max_q, exact, st);
-    if (d == 128) return launch_chunk<128>(a, p, B, max_q, exact, st);
-    return launch_chunk<256>(a, p, B, max_q, exact, st);
+    if (d == 64) return launch_chunk<64>(a, p, T, B, max_q, exact, st);
+    if (d == 128) return launch_chunk<128>(a, p, T, B, max_q, exact, st);
+    return launch_chunk<256>(a, p, T, B, max_q, exact, st);
 }

@@ -293,7 +293,7 @@ extern "C" int oom_attn_plan(const int32_t* cu_q, const int32_t* kv_lens, const 
     a.T = T;
     a.G = heads / kv_heads;
     a.Hkv = kv_heads;
-    a.few_rows = attn_few_rows(d);
+    a.few_rows = attn_has_few(T, B, a.G, d) ? attn_few_rows(d) : 0;
     a.split_blocks = attn_split_blocks(d);
     a.sign = attn_plan_sign(T, B, heads, kv_heads, d, page_table ? max_pages : 0, page_table ? page_size : 0);
     a.max_items = p.items;

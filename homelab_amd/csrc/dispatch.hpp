@@ -306,6 +306,9 @@ constexpr int ATTN_MAX_KEYS = 1 << 27;  // keys of a sequence
 // A sequence of at most so many packed rows over a paged cache is one tile of attn_few.hpp, whose
 // waves hold all of them: at d 256, Q and O of 32 rows would not fit a wave's registers.
 constexpr int attn_few_rows(int d) { return d == 256 ? 16 : 32; }
+// Whether a batch may have such sequences: a lone sequence is one only where the batch has no more
+// rows than that, so that its kind follows from sizes that the host knows.
+inline bool attn_has_few(int64_t T, int64_t B, int G, int d) { return B > 1 || T * G <= attn_few_rows(d); }
 
 // Blocks that the other sequences' keys are split for: as many as the chip holds at once, two a CU,
 // but one at d 256, whose tiles fill a CU's LDS (128 tokens over 8000 keys at 24/2 heads: 47 us

@@ -225,6 +225,32 @@ def test_plan_of_other_sizes_writes_nothing(hip):
         assert bool((out == 3.0).all())
 
 
+@pytest.mark.parametrize("d", [64, 256])
+@pytest.mark.parametrize("T,new,max_q", [(64, [1], 64), (64, [1], 1), (64, [40], 64), (3, [1], 50), (2, [2], 2), (1, [1], 900),
+                                         (70, [1, 2], 1000), (70, [60, 0], 64)])
+def test_bounds_above_the_lengths(hip, T, new, max_q, d):
+    """T and max_q are bounds (of a captured step's buffers): fewer tokens than either are served."""
+    g = pc.gen(T + max_q)
+    H, Hkv, page = 16, 2, 16
+    kv = [300 + n for n in new]
+    kp, vp, table = pc.paged(g, kv, Hkv, d, page)
+    q = pc.randn(g, (T, H, d), BF)
+    B = len(new)
+    plan = torch.zeros(hip.attn_plan_size(T, B, H, Hkv, d), dtype=torch.int32, device="cuda")
+    hip.attn_plan(pc.cumulative(new), torch.tensor(kv, dtype=torch.int32, device="cuda"), table, T, H, Hkv, d, plan,
+                  n_pages=kp.shape[0], page_size=page)
+    ws = torch.zeros(hip.attn_chunk_paged_workspace_size(T, B, H, Hkv, d), dtype=torch.uint8, device="cuda")
+    out = torch.full((T, H, d), 3.0, dtype=BF, device="cuda")
+    hip.attn_chunk_paged(q, kp, vp, table, plan, max(max_q, max(new)), 0.1, out, ws)
+    at = 0
+    for b, n in enumerate(new):
+        k, v = (pc.unpaged(x, table[b], kv[b], page) for x in (kp, vp))
+        want, tol = pc.attention(q[at:at + n], k, v, 0.1, kv[b] - n, False)
+        pc.hold(out[at:at + n], want, tol)
+        at += n
+    assert bool((out[at:] == 3.0).all())
+
+
 def test_lengths_past_the_table_and_sequences_that_share_pages(hip):
     """kv_lens past a sequence's pages are taken as its pages; two sequences may name the same pages."""
     g = pc.gen(17)
@@ -405,7 +431,8 @@ def test_plan_covers_every_row_and_key_once(hip, seed):
     for b, n in enumerate(new):
         for r0 in range(0, n * G, 128):
             r = min(128, n * G - r0)
-            tiles[(b, r0)] = (at, r, kv[b] - n, max(0, kv[b] - n + (r0 + r - 1) // G + 1), n * G <= few_rows)
+            few = n * G <= few_rows and (B > 1 or T * G <= few_rows)
+            tiles[(b, r0)] = (at, r, kv[b] - n, max(0, kv[b] - n + (r0 + r - 1) // G + 1), few)
         at += n
     seen, parts, merged = {}, {}, {}
     for few, items in ((False, one), (True, two)):

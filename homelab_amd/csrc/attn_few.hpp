@@ -27,13 +27,6 @@ __device__ __forceinline__ void f_wait_loads() {
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
-// This wave's LDS reads are done: what they read may be written over by loads.
-__device__ __forceinline__ void f_wait_reads() {
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0); vmcnt and expcnt left at their maxima
-    __atomic_signal_fence(__ATOMIC_SEQ_CST);
-}
-
 template <int D, int TERMS, int M>
 __device__ __forceinline__ void few_rows(const TileArgs& a, const AttnItem& it, int h, uint8_t* lds,
                                          float (&mlds)[few_waves<D>()][32], float (&llds)[few_waves<D>()][32]) {
@@ -117,7 +110,7 @@ __device__ __forceinline__ void few_rows(const TileArgs& a, const AttnItem& it, 
             t_wait_loads();
         }
         if (more) {
-            f_wait_reads();
+            t_wait_lds();
             load(t + 1, kb, ko, k_at);
         }
         const float mb = tile_maximum(s, c);
@@ -135,7 +128,7 @@ __device__ __forceinline__ void few_rows(const TileArgs& a, const AttnItem& it, 
         }
         tile_values(s, vt, c, mb, lane);
         if (more) {
-            f_wait_reads();
+            t_wait_lds();
             load(t + 1, vb, vo, v_at);
         }
     };

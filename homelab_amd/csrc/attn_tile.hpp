@@ -115,6 +115,13 @@ __device__ __forceinline__ void t_wait_loads() {
     __atomic_signal_fence(__ATOMIC_SEQ_CST);
 }
 
+// This wave's LDS reads and writes are done; its loads into LDS may be on their way.
+__device__ __forceinline__ void t_wait_lds() {
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+    __builtin_amdgcn_s_waitcnt(0xC07F);  // lgkmcnt(0); vmcnt and expcnt left at their maxima
+    __atomic_signal_fence(__ATOMIC_SEQ_CST);
+}
+
 // Where a run of keys lies in its page: byte offset from the head's first row of page 0, or -1 (a bad
 // page, or past the item's keys).
 __device__ __forceinline__ int64_t page_offset(const TileArgs& a, const int32_t* table, int key, int k1, int row_bytes) {
@@ -246,14 +253,16 @@ struct Mx<16> {
 // output's own rounding; the sum l is that of the rounded p). TERMS 3: fp32 on either side: Q
 // and P enter as three exact bf16 terms each (hi + mid + lo), so products are exact and only
 // fp32 sums round.
-template <int D, int TERMS, int M, int KEYS = ATTN_KEYS>
+// A wave scores KEYS keys of a tile and holds DO of the output's dims: all of both, but for pair_block().
+template <int D, int TERMS, int M, int KEYS = ATTN_KEYS, int DO = D>
 struct RowState {
     static constexpr int KD = 512 / M;    // dims (keys) a product sums over
     static constexpr int E = M * M / 64;  // elements of a result a lane
     static constexpr int NS = KEYS / M;   // results a tile of scores
+    static constexpr int NO = DO / M;     // results of the output
     typedef typename Mx<M>::acc acc;
     tbf16x8 q[TERMS][D / KD];
-    acc o[D / M];
+    acc o[NO];
     acc sc[NS];  // scores of the present tile
     float m, l;
     int pos;    // the last key this lane's row sees
@@ -263,8 +272,8 @@ struct RowState {
 template <int M>
 constexpr int score_key(int n, int i) { return M * n + (256 / M) * (i / 4) + i % 4; }
 
-template <int D, int TERMS, int M, int KEYS>
-__device__ __forceinline__ void rows_init(RowState<D, TERMS, M, KEYS>& s, const TileArgs& a, const AttnItem& it, int h, int wrow,
+template <int D, int TERMS, int M, int KEYS, int DO>
+__device__ __forceinline__ void rows_init(RowState<D, TERMS, M, KEYS, DO>& s, const TileArgs& a, const AttnItem& it, int h, int wrow,
                                           int lane) {
     const int r = wrow + lane % M, part = lane / M;
     s.live = r < it.rows;
@@ -273,7 +282,7 @@ __device__ __forceinline__ void rows_init(RowState<D, TERMS, M, KEYS>& s, const 
     s.m = -INFINITY;
     s.l = 0.0f;
 #pragma unroll
-    for (int d = 0; d < D / M; d++) s.o[d] = typename Mx<M>::acc{};
+    for (int d = 0; d < DO / M; d++) s.o[d] = typename Mx<M>::acc{};
     constexpr int KD = 512 / M;
     const int64_t at = (int64_t)(it.q0 + (int)tok) * a.q_stride + (int64_t)(h * a.G + (int)g) * D + 8 * part;
     if constexpr (TERMS == 1) {
@@ -318,10 +327,10 @@ __device__ __forceinline__ void rows_init(RowState<D, TERMS, M, KEYS>& s, const 
 // or past the item's keys (last: the last one that the lane's row sees). BAD_K, with three terms: K
 // holds infinities or NaN, which meet the first term alone; the others may be zero or of the
 // other sign. V holds none (the kernel takes them out).
-template <bool MASKED, bool BAD_K, int D, int TERMS, int M, int KEYS>
-__device__ __forceinline__ void tile_scores(RowState<D, TERMS, M, KEYS>& s, const uint8_t* kt, int last, int lane) {
+template <bool MASKED, bool BAD_K, int D, int TERMS, int M, int KEYS, int DO>
+__device__ __forceinline__ void tile_scores(RowState<D, TERMS, M, KEYS, DO>& s, const uint8_t* kt, int last, int lane) {
     typedef TileLay<D> L;
-    typedef RowState<D, TERMS, M, KEYS> S;
+    typedef RowState<D, TERMS, M, KEYS, DO> S;
     const int part = lane / M;
     const uint8_t* krow = kt + (lane % M) * L::ROWB;
     const int kx = L::kx(lane % M);  // rows M apart have the same
@@ -472,17 +481,18 @@ __device__ __forceinline__ void tile_values(RowState<D, TERMS, M, KEYS>& s, cons
 
 // The infinities and NaN of a V tile to the rows that see their key: a hidden key has no part in a
 // row, whatever its value holds, and its weight of zero times an infinity would be NaN.
-template <int D, int TERMS, int M, int KEYS>
-__device__ __forceinline__ void tile_bad_values(RowState<D, TERMS, M, KEYS>& s, const uint8_t* vt, int last, int lane) {
+template <int D, int TERMS, int M, int KEYS, int DO>
+__device__ __forceinline__ void tile_bad_values(RowState<D, TERMS, M, KEYS, DO>& s, const uint8_t* vt, int last, int lane,
+                                                int keys = KEYS, int dim0 = 0) {
     typedef TileLay<D> L;
     const int part = lane / M;
-    for (int key = 0; key < KEYS; key++) {
+    for (int key = 0; key < keys; key++) {
         if (!__any(key <= last)) break;
 #pragma unroll
-        for (int d = 0; d < D / M; d++)
+        for (int d = 0; d < DO / M; d++)
 #pragma unroll
             for (int e = 0; e < M * M / 256; e++) {
-                const int dim = M * d + (256 / M) * e + 4 * part;
+                const int dim = dim0 + M * d + (256 / M) * e + 4 * part;
                 const uint2 w = *reinterpret_cast<const uint2*>(vt + key * L::ROWB + 16 * ((dim / 8) ^ L::vx(key)) +
                                                                 2 * (dim & 7));
                 const uint32_t b0 = w.x & ~t_finite(w.x), b1 = w.y & ~t_finite(w.y);
@@ -507,48 +517,49 @@ __device__ __forceinline__ int64_t row_at(const TileArgs& a, const AttnItem& it,
 // which no wave reads any more) so that a store covers whole rows, 1 KB at a time; chunks of 16
 // bytes are permuted within a row against bank conflicts. (Stored from the registers, 8 or 16
 // bytes a row and instruction: 2 % slower on short prompts.)
-template <int D, int TERMS, int M>
-__device__ __forceinline__ void rows_store(RowState<D, TERMS, M>& s, const TileArgs& a, const AttnItem& it, int h, int wrow,
-                                           int lane, uint8_t* lds) {
+template <int D, int TERMS, int M, int KEYS, int DO>
+__device__ __forceinline__ void rows_store(RowState<D, TERMS, M, KEYS, DO>& s, const TileArgs& a, const AttnItem& it, int h,
+                                           int wrow, int lane, uint8_t* lds, int dim0 = 0) {
     const int r = lane % M, part = lane / M;
     s.l = row_sum<M>(s.l);
     const bool wide = it.part >= 0 || a.out_dtype == OOM_F32;  // uniform
     const int64_t pr = (int64_t)h * a.part_rows + it.part + wrow;
-    if (it.part >= 0 && part == 0 && s.live) *reinterpret_cast<float2*>(a.part_ml + 2 * (pr + r)) = make_float2(s.m, s.l);
+    if (it.part >= 0 && dim0 == 0 && part == 0 && s.live) *reinterpret_cast<float2*>(a.part_ml + 2 * (pr + r)) = make_float2(s.m, s.l);
     const float f = it.part >= 0 ? 1.0f : s.pos < 0 ? 0.0f : 1.0f / s.l;
 #pragma unroll
-    for (int d = 0; d < D / M; d++)
+    for (int d = 0; d < DO / M; d++)
 #pragma unroll
         for (int e = 0; e < M * M / 256; e++) {
             const float x0 = s.o[d][4 * e] * f, x1 = s.o[d][4 * e + 1] * f, x2 = s.o[d][4 * e + 2] * f,
                         x3 = s.o[d][4 * e + 3] * f;
             const int dim = M * d + 256 / M * e + 4 * part;
             if (wide)
-                *reinterpret_cast<float4*>(lds + r * D * 4 + 16 * ((dim / 4) ^ (r & 15))) = make_float4(x0, x1, x2, x3);
+                *reinterpret_cast<float4*>(lds + r * DO * 4 + 16 * ((dim / 4) ^ (r & 15))) = make_float4(x0, x1, x2, x3);
             else
-                *reinterpret_cast<uint2*>(lds + r * D * 2 + 16 * ((dim / 8) ^ (r & (D / 8 - 1) & 15)) + 2 * (dim & 7)) =
+                *reinterpret_cast<uint2*>(lds + r * DO * 2 + 16 * ((dim / 8) ^ (r & (DO / 8 - 1) & 15)) + 2 * (dim & 7)) =
                     make_uint2(t_pack(x0, x1), t_pack(x2, x3));
         }
     wave_lds_order();
     if (wide) {
-        constexpr int C = D / 4;  // chunks a row
+        constexpr int C = DO / 4;  // chunks a row
 #pragma unroll
         for (int i = 0; i < M * C / 64; i++) {
             const int row = (64 * i + lane) / C, ch = (64 * i + lane) % C;
             if (wrow + row >= it.rows) continue;
-            const float4 v = *reinterpret_cast<const float4*>(lds + row * D * 4 + 16 * (ch ^ (row & 15)));
+            const float4 v = *reinterpret_cast<const float4*>(lds + row * DO * 4 + 16 * (ch ^ (row & 15)));
             float* to = it.part >= 0 ? a.part_acc + (pr + row) * D
                                      : reinterpret_cast<float*>(a.out) + row_at(a, it, h, D, wrow + row);
-            *reinterpret_cast<float4*>(to + 4 * ch) = v;
+            *reinterpret_cast<float4*>(to + dim0 + 4 * ch) = v;
         }
     } else {
-        constexpr int C = D / 8;
+        constexpr int C = DO / 8;
 #pragma unroll
         for (int i = 0; i < M * C / 64; i++) {
             const int row = (64 * i + lane) / C, ch = (64 * i + lane) % C;
             if (wrow + row >= it.rows) continue;
-            const uint4 v = *reinterpret_cast<const uint4*>(lds + row * D * 2 + 16 * (ch ^ (row & (C - 1) & 15)));
-            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + row_at(a, it, h, D, wrow + row) + 8 * ch) = v;
+            const uint4 v = *reinterpret_cast<const uint4*>(lds + row * DO * 2 + 16 * (ch ^ (row & (C - 1) & 15)));
+            *reinterpret_cast<uint4*>(reinterpret_cast<uint16_t*>(a.out) + row_at(a, it, h, D, wrow + row) + dim0 + 8 * ch) =
+                v;
         }
     }
 }
@@ -622,7 +633,7 @@ __device__ __forceinline__ void tile_block(const TileArgs& a, uint32_t index, ui
         uint32_t* const bad = bad_lds + (stage ? 2 : 0);
         if (bk) bad[0] = 1;
         if (bv) bad[1] = 1;
-        __builtin_amdgcn_s_waitcnt(0xC07F);
+        t_wait_lds();
     };
     const auto step = [&](auto masked_tile) {
         constexpr bool MASKED = decltype(masked_tile)::value;
@@ -665,15 +676,205 @@ __device__ __forceinline__ void tile_block(const TileArgs& a, uint32_t index, ui
             make_float2(-INFINITY, 0.0f);
 }
 
-// Rows a wave: 32 up to d 128 in one term; 16 for three terms and for d 256, whose Q and O of 32 rows
-// leave no registers for a second wave on the SIMD. Waves a block: a tile's rows, but half of
-// them for three terms up to d 128, so that two blocks fit a CU and do not wait at the same
-// barriers (LDS holds one block at d 256).
+// d 256 in one term, whose 16-row waves above would each read the whole tile from LDS for half the
+// products: a pair of waves (w, w + 4) has 32 rows. Each scores half of the tile's keys, and their
+// weights meet in LDS; then each sums all keys' values into half of the dims. So a wave reads
+// half of K and half of V, and its Q and half of O leave room for two waves a SIMD. The pair
+// keeps the same maxima: the weights are taken with those of the tiles before, and only where a
+// row of the block outgrew its (by T_GROW; a row's first keys do) do the pairs exchange maxima
+// and take the weights again.
+// (2048 and 40 tokens at 24/2 heads: 74 us with 16-row waves, 67 so; a tile 1.7 us, 1.2 of it the chain
+// of barriers, LDS round trips and softmax between the products.)
+struct PairLds {
+    uint4 p[8][2][64];  // a wave's weights: the operands of its two products a tile
+    float mx[8][32];    // its rows' maxima, where some row's grew
+    uint32_t grew[2];   // some row's did, by the tile's parity
+    uint32_t bad[2];    // V holds infinities or NaN, by stage
+};
+
+// The N products before this are issued with their operands' LDS reads (R each) up to 6 products ahead.
+template <int N, int R>
+__device__ __forceinline__ void reads_ahead() {
+    constexpr int MFMA = 0x008, LDSR = 0x100, AHEAD = 6;
+    __builtin_amdgcn_sched_group_barrier(LDSR, R * AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < N - AHEAD; i++) {
+        __builtin_amdgcn_sched_group_barrier(MFMA, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(LDSR, R, 0);
+    }
+    __builtin_amdgcn_sched_group_barrier(MFMA, AHEAD, 0);
+}
+
+template <bool PAGED>
+__device__ __forceinline__ void pair_block(const TileArgs& a, uint32_t index, uint8_t* tiles, PairLds& x) {
+    constexpr int D = 256, M = 32, NW = 8, DO = D / 2;
+    typedef TileLay<D> L;
+    typedef RowState<D, 1, M, 32, DO> S;
+    const int lane = threadIdx.x & 63;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int h = (int)(index % (uint32_t)a.Hkv), item = (int)(index / (uint32_t)a.Hkv);
+    const AttnItem it = reinterpret_cast<const AttnItem*>(a.plan + ATTN_PLAN_HEAD)[item];
+    if (a.plan[ATTN_PLAN_SIGN] != a.plan_sign || item >= a.plan[ATTN_PLAN_ITEMS]) return;
+    const int part = wave / 4, wrow = M * (wave % 4);  // the wave's half of the keys, then of the dims
+    const bool has = wrow < it.rows;                   // uniform
+    const float c = a.scale * 1.44269504088896340736f;
+    TileSrc<D, NW, PAGED> src;
+    src.init(a, it, h, lane, wave);
+    if (threadIdx.x < 2) x.grew[threadIdx.x] = x.bad[threadIdx.x] = 0;
+    const uint32_t mine = (uint32_t)(uintptr_t)(t_lds_t)tiles + wave * (L::BYTES / NW);
+    if (it.k0 < it.k1) src.load(a, 0, lane, mine, mine + L::BYTES);
+    S s;
+    rows_init(s, a, it, h, wrow, lane);
+    __syncthreads();  // the flags are cleared
+    const int pos_hi = it.off + (int)((uint32_t)(it.row0 + min(wrow + M - 1, it.rows - 1)) / (uint32_t)a.G);
+    const int block_lo = it.off + (int)((uint32_t)it.row0 / (uint32_t)a.G);
+    const int whole = it.k0 + (max(0, min(it.k1, block_lo + 1) - it.k0) & ~63);
+    int key0 = it.k0;
+    uint32_t odd = 0;  // the tile's parity: its stage
+    // where a lane's first K chunk and V rows are in a tile of stage 0: chunks differ in bits 4 to 8 of the
+    // place, which the permutations combine by exclusive or, and the tiles are 32 KB each
+    const uint32_t k_at = (32 * part + lane % M) * L::ROWB + 16 * ((lane / M) ^ L::kx(lane % M));
+    const int vr = 4 * (lane / M) + ((lane & 15) >> 2);
+    const uint32_t v_at = L::BYTES + (32 * part + vr) * L::ROWB + 8 * (lane & 1) +
+                          16 * ((DO / 8 * part + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1)) ^ L::vx(vr));
+    tbf16x8 pb[2];
+    // p = 2^(s c - m c) of the wave's scores, for itself and for its partner
+    const auto weights = [&]() {
+        const float m0 = s.m == -INFINITY ? 0.0f : s.m, sub = c > 1.0f ? m0 : 0.0f, mb = c > 1.0f ? 0.0f : m0 * c;
+#pragma unroll
+        for (int w = 0; w < 2; w++) {
+            uint32_t b[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float s0 = s.sc[0][8 * w + 2 * j], s1 = s.sc[0][8 * w + 2 * j + 1];
+                b[j] = t_pack(__builtin_amdgcn_exp2f(fmaf(s0 - sub, c, -mb)), __builtin_amdgcn_exp2f(fmaf(s1 - sub, c, -mb)));
+            }
+            const uint4 v = make_uint4(b[0], b[1], b[2], b[3]);
+            pb[w] = __builtin_bit_cast(tbf16x8, v);
+            x.p[wave][w][lane] = v;
+        }
+    };
+    const auto step = [&](auto masked_tile) {
+        constexpr bool MASKED = decltype(masked_tile)::value;
+        uint8_t* const vt = tiles + odd * (2 * L::BYTES) + L::BYTES;
+        t_wait_loads();
+        if constexpr (MASKED) {  // V's infinities and NaN in the wave's part of the tile
+            uint32_t bv = 0;
+#pragma unroll
+            for (int n = 0; n < L::BYTES / NW / 1024; n++) {
+                const uint4 w = *reinterpret_cast<const uint4*>(vt + wave * (L::BYTES / NW) + n * 1024 + 16 * lane);
+                bv |= t_nonfinite(w.x) | t_nonfinite(w.y) | t_nonfinite(w.z) | t_nonfinite(w.w);
+            }
+            if (bv) x.bad[odd] = 1;
+            t_wait_lds();
+        }
+        t_barrier();
+        if (key0 + 64 < it.k1) {
+            const uint32_t to = mine + (odd ^ 1) * (2 * L::BYTES);
+            src.load(a, (key0 + 64 - it.k0) / 64, lane, to, to + L::BYTES);
+        }
+        const bool sees = has && (!MASKED || key0 <= pos_hi);  // uniform, and the same for the pair
+        const int last = MASKED ? min(s.pos, it.k1 - 1) - key0 : 63;
+        float mx = -INFINITY;
+        if (sees) {
+            s.sc[0] = typename S::acc{};
+#pragma unroll
+            for (int st = 0; st < D / S::KD; st++) {
+                const tbf16x8 k8 = *reinterpret_cast<const tbf16x8*>(tiles + (k_at ^ (odd * (2 * L::BYTES)) ^ 32 * st));
+                s.sc[0] = Mx<M>::mul(k8, s.q[0][st], s.sc[0]);
+            }
+            reads_ahead<D / S::KD, 1>();
+            if constexpr (MASKED) {
+#pragma unroll
+                for (int i = 0; i < S::E; i++)
+                    if (score_key<M>(part, i) + 4 * (lane / M) > last) s.sc[0][i] = -INFINITY;
+            }
+#pragma unroll
+            for (int i = 0; i < S::E; i++) mx = fmaxf(mx, s.sc[0][i]);
+            mx = row_max<M>(mx);
+            if (__any((mx - s.m) * c > T_GROW)) x.grew[odd] = 1;
+            weights();
+        }
+        if (threadIdx.x == 0) x.grew[odd ^ 1] = 0;  // read before this tile's first barrier, set past the next's
+        t_wait_lds();
+        t_barrier();
+        if (x.grew[odd]) {  // uniform over the block; rare
+            if (sees && lane < M) x.mx[wave][lane] = mx;
+            t_wait_lds();
+            t_barrier();
+            if (sees) {
+                const float mn = fmaxf(s.m, fmaxf(mx, x.mx[wave ^ 4][lane % M]));
+                const float f = mn == -INFINITY ? 1.0f : __builtin_amdgcn_exp2f((s.m - mn) * c);
+                s.m = mn;
+                s.l *= f;
+#pragma unroll
+                for (int d = 0; d < S::NO; d++)
+#pragma unroll
+                    for (int i = 0; i < S::E; i++) s.o[d][i] *= f;
+                weights();
+            }
+            t_wait_lds();
+            t_barrier();
+        }
+        if (MASKED && x.bad[odd]) {  // uniform over the block; rare
+            if (sees) tile_bad_values(s, vt, last, lane, ATTN_KEYS, DO * part);
+            __syncthreads();
+#pragma unroll
+            for (int n = 0; n < L::BYTES / NW / 1024; n++) {
+                uint4* p = reinterpret_cast<uint4*>(vt + wave * (L::BYTES / NW) + n * 1024 + 16 * lane);
+                *p = __builtin_bit_cast(uint4, t_finite8(__builtin_bit_cast(tbf16x8, *p)));
+            }
+            if (threadIdx.x == 0) x.bad[odd] = 0;
+            __syncthreads();
+        }
+        if (sees) {
+            const tbf16x2 ones = __builtin_bit_cast(tbf16x2, 0x3f803f80u);
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                const uint4 v = __builtin_bit_cast(uint4, pb[w]);
+                for (const uint32_t b : {v.x, v.y, v.z, v.w})
+                    s.l = __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(tbf16x2, b), ones, s.l, false);
+            }
+            // 16 keys a product: those of the wave's own half, then its partner's
+            tbf16x8 p2[2];
+#pragma unroll
+            for (int w = 0; w < 2; w++) p2[w] = __builtin_bit_cast(tbf16x8, x.p[wave ^ 4][w][lane]);
+#pragma unroll
+            for (int w = 0; w < 4; w++)
+#pragma unroll
+                for (int d = 0; d < S::NO; d++) {
+                    const uint8_t* va = tiles + ((v_at ^ (odd * (2 * L::BYTES)) ^ 64 * d) ^ (w < 2 ? 0 : 32 * L::ROWB)) +
+                                        16 * (w % 2) * L::ROWB;
+                    const uint2 w0 = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)va));
+                    const uint2 w1 =
+                        __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((tr_ptr_t)(va + 8 * L::ROWB)));
+                    s.o[d] = Mx<M>::mul(__builtin_bit_cast(tbf16x8, make_uint4(w0.x, w0.y, w1.x, w1.y)),
+                                        w < 2 ? pb[w] : p2[w - 2], s.o[d]);
+                }
+            reads_ahead<4 * S::NO, 2>();
+        }
+    };
+    for (; key0 < whole; key0 += 64, odd ^= 1) step(std::false_type{});
+    for (; key0 < it.k1; key0 += 64, odd ^= 1) step(std::true_type{});
+    __syncthreads();  // every wave is done with the tiles and the weights
+    float* const sums = reinterpret_cast<float*>(x.p);
+    sums[64 * wave + lane] = s.l;
+    __syncthreads();
+    s.l += sums[64 * (wave ^ 4) + lane];
+    static_assert(4 * L::BYTES >= NW * M * DO * 4, "the rows fit the tiles' places");
+    if (has) rows_store(s, a, it, h, wrow, lane, tiles + wave * (M * DO * 4), DO * part);
+}
+
+// Rows a wave: 32 in one term (d 256: pair_block()), 16 for three terms, whose Q of 32 rows leaves no
+// registers for a second wave on the SIMD. Waves a block: a tile's rows, but half of them for
+// three terms up to d 128, so that two blocks fit a CU and do not wait at the same barriers (LDS
+// holds one block at d 256).
 template <int D, int TERMS>
 struct TileShape {
-    static constexpr int M = D <= 128 && TERMS == 1 ? 32 : 16;
+    static constexpr bool PAIRS = D == 256 && TERMS == 1;
+    static constexpr int M = TERMS == 1 ? 32 : 16;
     static constexpr int NW = D <= 128 ? 4 : 8;  // 64 NW threads: tile_threads()
-    static constexpr int PARTS = ATTN_ROWS / (M * NW);  // blocks a tile
+    static constexpr int PARTS = PAIRS ? 1 : ATTN_ROWS / (M * NW);  // blocks a tile
 };
 
 template <int D>
@@ -683,8 +884,13 @@ template <int D, int TERMS, bool PAGED>
 __global__ void __launch_bounds__(tile_threads<D>(), 2) attn_tile_kernel(TileArgs a) {
     typedef TileShape<D, TERMS> S;
     __shared__ __align__(16) uint8_t tiles[tile_lds<D>()];
-    __shared__ uint32_t bad_lds[4];
-    tile_block<D, TERMS, S::M, S::NW, PAGED>(a, blockIdx.x, tiles, bad_lds);
+    if constexpr (S::PAIRS) {
+        __shared__ PairLds pairs;
+        pair_block<PAGED>(a, blockIdx.x, tiles, pairs);
+    } else {
+        __shared__ uint32_t bad_lds[4];
+        tile_block<D, TERMS, S::M, S::NW, PAGED>(a, blockIdx.x, tiles, bad_lds);
+    }
 }
 
 template <int D, int TERMS, bool PAGED>

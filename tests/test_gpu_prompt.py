@@ -210,3 +210,57 @@ def test_chunk_one_token_agrees_with_decode(hip):
     k, v = (pc.unpaged(x, table[0], kv, page) for x in (kp, vp))
     _, tol = pc.attention(q, k, v, 0.088, kv - 1, True)
     assert bool(((out[0] - one).double().abs() <= 2 * tol[0] + 1e-7).all())
+
+
+@pytest.mark.parametrize("scale", [0.25, 1.0])
+@pytest.mark.parametrize("d,qdt", [(64, BF), (128, BF), (256, BF), (64, F32), (128, F32), (256, F32)])
+def test_maxima_that_grow_from_tile_to_tile(hip, d, qdt, scale):
+    """Scores that rise along the keys for some rows, fall for others and stay for the rest: the running
+    maximum moves in every tile, for a part of a wave's rows; scales on both sides of ln 2."""
+    g = pc.gen(41 + d)
+    T, H, Hkv, page = 390, 6, 2, 16
+    q = 0.1 * pc.randn(g, (T, H, d))
+    q[:, :, 0] = torch.randint(-1, 2, (T, H), generator=g, device="cuda").float()
+    k, v = (0.1 * pc.randn(g, (T, Hkv, d))).to(BF), pc.randn(g, (T, Hkv, d), BF)
+    k[:, :, 0] = (torch.arange(T, device="cuda") // 8 * 4.0).to(BF)[:, None]
+    q = q.to(qdt)
+    check_prompt(hip, q, k, v, [T - 50, 47], scale, qdt)
+    # the same keys in pages: many new tokens (split over the keys), few, one
+    kp, vp, table = pc.paged(g, [T] * 3, Hkv, d, page)
+    for b in range(3):
+        for i in range(0, T, page):
+            n = min(page, T - i)
+            kp[int(table[b, i // page]), :, :n] = k[i:i + n].transpose(0, 1)
+            vp[int(table[b, i // page]), :, :n] = v[i:i + n].transpose(0, 1)
+    check_chunk(hip, q[:96], kp, vp, table, [90, 4, 1], [T, T - 3, T], scale, qdt)
+
+
+@pytest.mark.parametrize("d,qdt", [(128, BF), (256, BF), (128, F32), (256, F32)])
+def test_prompt_large_scores_of_wide_heads(hip, d, qdt):
+    """test_prompt_large_scores at the other head sizes and fp32 queries."""
+    g = pc.gen(43)
+    T, H = 190, 2
+    q = torch.zeros((T, H, d), dtype=qdt, device="cuda")
+    q[:, :, 0] = 1.0
+    k = torch.zeros((T, 1, d), dtype=BF, device="cuda")
+    k[:, 0, 0] = -3.0e38
+    k[60:, 0, 0] = torch.randint(-100, 100, (T - 60,), generator=g, device="cuda").to(BF)
+    check_prompt(hip, q, k, pc.randn(g, (T, 1, d), BF), [T], 1.0, qdt)
+
+
+@pytest.mark.parametrize("d,qdt", [(64, BF), (256, BF), (64, F32), (128, F32), (256, F32)])
+def test_chunk_bad_pages_and_infinities_of_every_kernel(hip, d, qdt):
+    """Bad pages in the first, a middle and the last tile; infinities and NaN seen by some, all and no rows; of
+    a sequence of many rows and of one of few."""
+    g = pc.gen(44 + d)
+    new, kv, H, Hkv, page = [70, 2], [400, 500], 4, 2, 16
+    kp, vp, table = pc.paged(g, kv, Hkv, d, page)
+    vp[int(table[0, 23]), 0, 3, 9] = math.inf    # key 371 of sequence 0: seen from its token 41 on
+    vp[int(table[0, 2]), 1, 0, d - 1] = math.nan  # key 32: seen by all
+    vp[int(table[1, 31]), 0, 3, 2] = -math.inf   # key 499: seen by the last token alone
+    kp[int(table[1, 31]), 1, 3, 2] = math.nan
+    table[0, 0], table[0, 9], table[0, 24], table[1, 0], table[1, 17] = -1, kp.shape[0], 1 << 30, -(1 << 31), 1 << 30
+    q = pc.randn(g, (sum(new), H, d), qdt)
+    out = check_chunk(hip, q, kp, vp, table, new, kv, 0.09, qdt)
+    assert bool(out[:41, :2].isfinite().all()) and bool(out[41:70, :2, 9].isinf().all())
+    assert bool(out[70].isfinite().all()) and bool(out[71, 2:].isnan().all())

@@ -152,10 +152,10 @@ __global__ void __launch_bounds__(PLAN_THREADS) attn_plan_kernel(PlanArgs a) {
     }
     __syncthreads();
     // Units a split. Prompts are not split: their rows alone fill the chip, or their keys are few. Else
-    // the work's even share a block, or up to a quarter more where that keeps the splits to as many
+    // the work's even share a block, or up to a half more where that keeps the splits to as many
     // blocks as run at once, so that no few of them make a second round (512 tokens over 16 Ki
-    // keys, d 128: 284 us with the share, 275 so; with no bound on the share, 3 x 300 tokens over
-    // up to 3000 keys at d 256 took 104 us, not 71).
+    // keys, d 128: 284 us with the share, 275 so; over 8000 keys at d 256: 148 with a quarter more at
+    // most, 135 so; with no bound, 3 x 300 tokens over up to 3000 keys at d 256 took 104 us, not 71).
     int ks[2] = {longest[0], longest[1]};
     if (a.kv_lens) {
         PlanTile p = {};
@@ -167,7 +167,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) attn_plan_kernel(PlanArgs a) {
             ks[f] = share;
             // (more tiles than threads are more than the blocks: no search)
             if (tiles > PLAN_THREADS) continue;
-            for (int k = share; k <= share + share / 4 && k < longest[f]; k += max(1, share / 16)) {
+            for (int k = share; k <= share + share / 2 && k < longest[f]; k += max(1, share / 16)) {
                 int all;
                 block_scan(p.rows > 0 && p.few == (f == 1) ? (p.n + k - 1) / k : 0, tmp, all);
                 if ((int64_t)all * a.Hkv <= slots) {

@@ -311,8 +311,8 @@ constexpr int attn_few_rows(int d) { return d == 256 ? 16 : 32; }
 inline bool attn_has_few(int64_t T, int64_t B, int G, int d) { return B > 1 || T * G <= attn_few_rows(d); }
 
 // Blocks that the other sequences' keys are split for: as many as the chip holds at once, two a CU,
-// but one at d 256, whose tiles fill a CU's LDS (128 tokens over 8000 keys at 24/2 heads: 47 us
-// with 256 blocks, 58 with 512; at d 128, 64/8 heads, 512 over 16 Ki keys: 350 with 256, 300 with 512).
+// but one at d 256, whose tiles fill a CU's LDS (128 tokens over 8000 keys at 24/2 heads: 46 us
+// with 256 blocks, 61 with 512; at d 128, 64/8 heads, 512 over 16 Ki keys: 350 with 256, 300 with 512).
 constexpr int attn_split_blocks(int d) { return d == 256 ? 256 : 512; }
 
 // A plan in i32 words: ATTN_PLAN_HEAD words of counts, then the items, the few-row sequences' items,

@@ -403,7 +403,9 @@ int oom_attn_decode_turbo(const float* q, const uint8_t* k, const uint8_t* v, in
  * Tokens are packed: token rows of sequence b are [cu_q[b], cu_q[b + 1]) of T, rows at or past
  * cu_q[B] belong to none and stay as they were. Strides are in elements, between tokens, so q, k
  * and v may be slices of one fused projection's rows: multiples of 8, every base 16-byte
- * aligned. None of these calls keeps state: a workspace needs no fill. */
+ * aligned. None of these calls keeps state: a workspace needs no fill, and may be shared by calls
+ * (and captured graphs) that follow each other on a stream; calls that overlap in time need
+ * one each, and may share a plan. */
 
 /* Which dims of a head form a pair, among its first rot_dim: (i, i + rot_dim / 2) or (2i, 2i + 1). */
 #define OOM_ROPE_HALF 0

@@ -194,6 +194,40 @@ def test_on_another_stream(hip):
     pc.hold(out, want, tol)
 
 
+@pytest.mark.parametrize("d", [64, 256])
+def test_two_calls_at_once_share_a_plan(hip, d):
+    """Two layers' chunk attention on two streams: one plan, a workspace each; q and out slices of wider rows."""
+    g = pc.gen(22 + d)
+    H, Hkv, page, new, kv = 8, 2, 16, [90, 1, 3], [2000, 1500, 700]
+    T = sum(new)
+    plan = torch.zeros(hip.attn_plan_size(T, 3, H, Hkv, d), dtype=torch.int32, device="cuda")
+    layers = []
+    for i in range(2):
+        kp, vp, t = pc.paged(g, kv, Hkv, d, page)
+        table = t if i == 0 else layers[0][2]
+        if i:  # the second layer's pages lie where the first's do
+            kp, vp = (torch.nan_to_num(x) for x in (kp, vp))
+        rows = pc.randn(g, (T, H + 3, d), BF)
+        ws = torch.full((hip.attn_chunk_paged_workspace_size(T, 3, H, Hkv, d),), 0xFF, dtype=torch.uint8, device="cuda")
+        layers.append((kp, vp, table, rows, torch.full((T, H + 2, d), 3.0, dtype=BF, device="cuda"), ws))
+    hip.attn_plan(pc.cumulative(new), torch.tensor(kv, dtype=torch.int32, device="cuda"), layers[0][2], T, H, Hkv, d, plan,
+                  n_pages=layers[0][0].shape[0], page_size=page)
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in layers]
+    for _ in range(3):
+        for st, (kp, vp, table, rows, out, ws) in zip(streams, layers):
+            hip.attn_chunk_paged(rows[:, 2:H + 2], kp, vp, table, plan, max(new), 0.1, out[:, 1:H + 1], ws, stream=st)
+    torch.cuda.synchronize()
+    for kp, vp, table, rows, out, ws in layers:
+        at = 0
+        for b, n in enumerate(new):
+            k, v = (pc.unpaged(x, table[b], kv[b], page) for x in (kp, vp))
+            want, tol = pc.attention(rows[at:at + n, 2:H + 2], k, v, 0.1, kv[b] - n, False)
+            pc.hold(out[at:at + n, 1:H + 1], want, tol)
+            at += n
+        assert bool((out[:, 0] == 3.0).all()) and bool((out[:, H + 1] == 3.0).all())
+
+
 def test_plan_of_other_sizes_writes_nothing(hip):
     """A plan that was made for another batch, for prompts, or never made leaves the outputs as they were."""
     g = pc.gen(16)

@@ -683,8 +683,8 @@ __device__ __forceinline__ void tile_block(const TileArgs& a, uint32_t index, ui
 // keeps the same maxima: the weights are taken with those of the tiles before, and only where a
 // row of the block outgrew its (by T_GROW; a row's first keys do) do the pairs exchange maxima
 // and take the weights again.
-// (2048 and 40 tokens at 24/2 heads: 74 us with 16-row waves, 67 so; a tile 1.7 us, 1.2 of it the chain
-// of barriers, LDS round trips and softmax between the products.)
+// (2048 and 40 tokens at 24/2 heads: 74 us with 16-row waves, 67 so. A tile takes 1.7 us a CU, and 1.2
+// with its products left out: the issue of its loads, barriers, LDS round trips and softmax.)
 struct PairLds {
     uint4 p[8][2][64];  // a wave's weights: the operands of its two products a tile
     float mx[8][32];    // its rows' maxima, where some row's grew
